@@ -498,6 +498,91 @@ int equigspr_match_descriptors(const float* src_desc, int32_t n_src, const float
 int equigspr_correspondence_labels(const float* src_pts, const float* tgt_pts, const int64_t* corr, int32_t n_corr,
                                    const float* gt_pose, float inlier_threshold, int32_t* labels, float* dist, void* stream);
 
+/* ---- context operators: what a block that lets the points of clouds see each other is made of -------------------
+ * No counterpart in the reference's scripts (its CrossAttentionPoseRegression has no attention layer); defined by the formulas here.
+ * Tensors are fp32, bf16 or fp16 (all operands of one call alike); products, softmax statistics, sums and norms are fp32 or wider.
+ * Additions to ABI 14: no earlier entry changed. */
+#define EQUIGSPR_F32  0
+#define EQUIGSPR_BF16 1
+#define EQUIGSPR_F16  2
+
+/* [batch, points, heads, dim] with unit stride in dim; strides in elements (0 for a broadcast axis) */
+typedef struct equigspr_attention_tensor {
+    void*   data;
+    int64_t stride_batch, stride_point, stride_head;
+} equigspr_attention_tensor;
+
+/* out = softmax over the allowed keys (scale Q K^T) V.  Key j is allowed for point i of sample b when i < q_lens[b], j < kv_lens[b],
+ * key_mask[b][j] != 0 and, if causal, j - kv_lens[b] <= i - q_lens[b] (the last point sees every key).  heads is a multiple of kv_heads:
+ * query head h reads key head h / (heads / kv_heads).  1 <= dim <= 128, scale > 0.  Lengths are clamped to [0, nq] / [0, nk]; null = all.
+ * Rows without an allowed key, and rows at or behind q_lens[b], give zeros.  Values of keys that are not allowed are never used. */
+typedef struct equigspr_attention {
+    int32_t dtype, batch, nq, nk, heads, kv_heads, dim, causal;
+    float   scale;
+    equigspr_attention_tensor q, k, v;
+    const int32_t* q_lens;      /* [batch] or null */
+    const int32_t* kv_lens;     /* [batch] or null */
+    const uint8_t* key_mask;    /* [batch, nk], rows mask_stride bytes apart, or null */
+    int64_t mask_stride;
+} equigspr_attention;
+
+/* out [batch, nq, heads, dim] contiguous; lse (optional, for the backward) [batch, kv_heads, nq * heads / kv_heads] floats;
+ * work: equigspr_attention_work_size floats (0: may be null) */
+int64_t equigspr_attention_work_size(const equigspr_attention* desc);
+int equigspr_attention_forward(const equigspr_attention* desc, void* out, float* lse, float* work, void* stream);
+/* out, lse: as the forward wrote them; grad_q / grad_k / grad_v: contiguous, written (not accumulated), each may be null.
+ * No atomics: results do not depend on timing. */
+int64_t equigspr_attention_backward_work_size(const equigspr_attention* desc);
+int equigspr_attention_backward(const equigspr_attention* desc, const void* out, const float* lse, const equigspr_attention_tensor* grad_out,
+                                float* work, void* grad_q, void* grad_k, void* grad_v, void* stream);
+
+#define EQUIGSPR_ACT_SILU 0
+#define EQUIGSPR_ACT_GELU 1     /* z Phi(z), the exact form */
+#define EQUIGSPR_ACT_RELU 2
+
+/* y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down.  x [rows, width], w_gate / w_up [hidden, width],
+ * w_down [out, hidden], all contiguous and of one dtype; biases of the same dtype, each may be null. */
+typedef struct equigspr_gated_feed_forward {
+    int32_t dtype, activation, rows, width, hidden, out;
+    const void *x, *w_gate, *w_up, *w_down, *b_gate, *b_up, *b_down;
+} equigspr_gated_feed_forward;
+/* written (not accumulated), each may be null.  grad_w_gate_up [2 * hidden, width]: the gate's rows, then the other projection's;
+ * grad_b_gate_up [2 * hidden] alike */
+typedef struct equigspr_gated_feed_forward_grads {
+    void *grad_x, *grad_w_gate_up, *grad_w_down, *grad_b_gate_up, *grad_b_down;
+} equigspr_gated_feed_forward_grads;
+/* y [rows, out]; h [rows, hidden] scratch of the inputs' dtype; zu [rows, 2 * hidden] or null: both projections, kept for the backward;
+ * work: ..._work_size floats (0: may be null) */
+int64_t equigspr_gated_feed_forward_work_size(const equigspr_gated_feed_forward* desc);
+int equigspr_gated_feed_forward_forward(const equigspr_gated_feed_forward* desc, void* y, void* h, void* zu, float* work, void* stream);
+/* grad_y [rows, out] contiguous; zu as the forward wrote it; h [rows, hidden] and dzu [rows, 2 * hidden]: scratch of the inputs' dtype */
+int64_t equigspr_gated_feed_forward_backward_work_size(const equigspr_gated_feed_forward* desc);
+int equigspr_gated_feed_forward_backward(const equigspr_gated_feed_forward* desc, const void* grad_y, const void* zu, void* h, void* dzu, float* work,
+                                         const equigspr_gated_feed_forward_grads* grads, void* stream);
+
+/* The residual step between two blocks, with the norm behind the first and the norm before the second:
+ *   z = post_weight ? norm(f) * post_weight + post_bias : f,   y = x + factor' * gate * z,   u = norm(y) * pre_weight + pre_bias,
+ * norm(v) = (v - mean) / sqrt(var + eps), or v / sqrt(mean(v^2) + eps) if rms; factor' = scale[c] when given, else factor.
+ * x, f [rows, width]; gate [rows / gate_rows, width] or null, of the same dtype; weights, biases and scale fp32 [width], each may be
+ * null (pre_weight null: no second norm, u is not written).  f null: y = x (y may be null), only u is formed.  1 <= width <= 8192. */
+typedef struct equigspr_residual_norm {
+    int32_t dtype, width, rms, reserved;
+    int64_t rows, gate_rows;
+    float   eps, factor;
+    const void *x, *f, *gate;
+    const float *post_weight, *post_bias, *pre_weight, *pre_bias, *scale;
+} equigspr_residual_norm;
+/* written (not accumulated), each may be null; grad_gate has the gate's shape and dtype */
+typedef struct equigspr_residual_norm_grads {
+    void *grad_x, *grad_f, *grad_gate;
+    float *grad_post_weight, *grad_post_bias, *grad_pre_weight, *grad_pre_bias, *grad_scale;
+} equigspr_residual_norm_grads;
+int equigspr_residual_norm_forward(const equigspr_residual_norm* desc, void* y, void* u, void* stream);
+/* grad_y, grad_u: either may be null (zeros); work: equigspr_residual_norm_backward_work_size floats.  The norms are recomputed from x and f. */
+int64_t equigspr_residual_norm_backward_work_size(const equigspr_residual_norm* desc);
+int equigspr_residual_norm_backward(const equigspr_residual_norm* desc, const void* grad_y, const void* grad_u, float* work,
+                                    const equigspr_residual_norm_grads* grads, void* stream);
+
 /* ---- measurement hooks (bench.py's roofline leg; NOT part of the drop-in path) -----------
  * Average duration in ms (written to HOST memory) of the EGNN message-passing edge kernel,
  * measured with HIP events on `stream` over `iters` back-to-back launches (these two calls

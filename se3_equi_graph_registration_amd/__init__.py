@@ -22,6 +22,10 @@ from .sh import (get_basis, get_spherical_harmonics, precompute_sh, basis_transf
                  wigner_d_matrix, compose, J_dense)
 from .gcn import build_graph, GraphConvolution, GlobalPooling, KnnAdjacency  # noqa: F401
 from .irreps import IrrepConv, IrrepEGNN, IrrepGNN, sh1_matrix  # noqa: F401  (N4: typed irrep-basis message passing)
+from .attention import cloud_attention, CloudAttention  # noqa: F401  (context operators: attention between the points of clouds)
+from .feedforward import gated_feed_forward, GatedFeedForward  # noqa: F401
+from .norms import residual_norm, ResidualNorm  # noqa: F401
+from .context import CloudContext  # noqa: F401  (blocks of the three between the EGNN and the pose head)
 from . import datasets  # noqa: F401  (N3: pair-file formats, dataset classes, HBM-resident batches)
 from . import train  # noqa: F401  (train_one_epoch / validate / checkpoints in the reference layout)
 from .datasets import ThreeDMatchTrainVal, ThreeDMatchTest, KITTItrainVal, KITTItest, DeviceBatches  # noqa: F401
@@ -29,4 +33,5 @@ from .datasets import ThreeDMatchTrainVal, ThreeDMatchTest, KITTItrainVal, KITTI
 __all__ = ["EGNN", "E_GCL", "CrossAttentionPoseRegression", "knn_graph", "get_edges_batch", "get_edges_from_idx",
            "build_pair_graph", "DeviceGraph", "weighted_kabsch", "pose_loss", "registration_loss", "compute_losses", "egnn_equi_loss",
            "unsorted_segment_sum", "unsorted_segment_mean", "synthetic_pair", "synthetic_batch", "SO3TensorProductLayer", "FlatAdam", "build_graph", "GraphConvolution",
-           "GlobalPooling", "KnnAdjacency", "IrrepConv", "IrrepGNN", "ThreeDMatchTrainVal", "ThreeDMatchTest", "KITTItrainVal", "KITTItest", "DeviceBatches"]
+           "GlobalPooling", "KnnAdjacency", "IrrepConv", "IrrepGNN", "cloud_attention", "CloudAttention",
+           "gated_feed_forward", "GatedFeedForward", "residual_norm", "ResidualNorm", "CloudContext", "ThreeDMatchTrainVal", "ThreeDMatchTest", "KITTItrainVal", "KITTItest", "DeviceBatches"]

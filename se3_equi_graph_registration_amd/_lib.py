@@ -39,6 +39,38 @@ class IrrepGnnConfig(Structure):
                 ("k11_0", ctypes.c_float), ("k11_1", ctypes.c_float), ("k11_2", ctypes.c_float)]
 
 
+class AttentionTensor(Structure):
+    _fields_ = [("data", c_void_p), ("stride_batch", c_int64), ("stride_point", c_int64), ("stride_head", c_int64)]
+
+
+class Attention(Structure):
+    _fields_ = [("dtype", c_int32), ("batch", c_int32), ("nq", c_int32), ("nk", c_int32), ("heads", c_int32), ("kv_heads", c_int32),
+                ("dim", c_int32), ("causal", c_int32), ("scale", ctypes.c_float), ("q", AttentionTensor), ("k", AttentionTensor),
+                ("v", AttentionTensor), ("q_lens", c_void_p), ("kv_lens", c_void_p), ("key_mask", c_void_p), ("mask_stride", c_int64)]
+
+
+class GatedFeedForward(Structure):
+    _fields_ = [("dtype", c_int32), ("activation", c_int32), ("rows", c_int32), ("width", c_int32), ("hidden", c_int32), ("out", c_int32),
+                ("x", c_void_p), ("w_gate", c_void_p), ("w_up", c_void_p), ("w_down", c_void_p), ("b_gate", c_void_p), ("b_up", c_void_p),
+                ("b_down", c_void_p)]
+
+
+class GatedFeedForwardGrads(Structure):
+    _fields_ = [("grad_x", c_void_p), ("grad_w_gate_up", c_void_p), ("grad_w_down", c_void_p), ("grad_b_gate_up", c_void_p),
+                ("grad_b_down", c_void_p)]
+
+
+class ResidualNorm(Structure):
+    _fields_ = [("dtype", c_int32), ("width", c_int32), ("rms", c_int32), ("reserved", c_int32), ("rows", c_int64), ("gate_rows", c_int64),
+                ("eps", ctypes.c_float), ("factor", ctypes.c_float), ("x", c_void_p), ("f", c_void_p), ("gate", c_void_p),
+                ("post_weight", c_void_p), ("post_bias", c_void_p), ("pre_weight", c_void_p), ("pre_bias", c_void_p), ("scale", c_void_p)]
+
+
+class ResidualNormGrads(Structure):
+    _fields_ = [("grad_x", c_void_p), ("grad_f", c_void_p), ("grad_gate", c_void_p), ("grad_post_weight", c_void_p),
+                ("grad_post_bias", c_void_p), ("grad_pre_weight", c_void_p), ("grad_pre_bias", c_void_p), ("grad_scale", c_void_p)]
+
+
 _SIGNATURES = {
     "equigspr_abi_version": (ctypes.c_int, []),
     "equigspr_last_error": (c_char_p, []),
@@ -115,6 +147,17 @@ _SIGNATURES = {
     "equigspr_step_loss_backward": (ctypes.c_int, [c_void_p] * 4 + [c_int32] + [c_void_p] * 3),
     "equigspr_match_descriptors": (ctypes.c_int, [c_void_p, c_int32, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
     "equigspr_correspondence_labels": (ctypes.c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p, ctypes.c_float, c_void_p, c_void_p, c_void_p]),
+    "equigspr_attention_work_size": (c_int64, [POINTER(Attention)]),
+    "equigspr_attention_forward": (ctypes.c_int, [POINTER(Attention)] + [c_void_p] * 4),
+    "equigspr_attention_backward_work_size": (c_int64, [POINTER(Attention)]),
+    "equigspr_attention_backward": (ctypes.c_int, [POINTER(Attention), c_void_p, c_void_p, POINTER(AttentionTensor)] + [c_void_p] * 5),
+    "equigspr_gated_feed_forward_work_size": (c_int64, [POINTER(GatedFeedForward)]),
+    "equigspr_gated_feed_forward_forward": (ctypes.c_int, [POINTER(GatedFeedForward)] + [c_void_p] * 5),
+    "equigspr_gated_feed_forward_backward_work_size": (c_int64, [POINTER(GatedFeedForward)]),
+    "equigspr_gated_feed_forward_backward": (ctypes.c_int, [POINTER(GatedFeedForward)] + [c_void_p] * 5 + [POINTER(GatedFeedForwardGrads), c_void_p]),
+    "equigspr_residual_norm_forward": (ctypes.c_int, [POINTER(ResidualNorm)] + [c_void_p] * 3),
+    "equigspr_residual_norm_backward_work_size": (c_int64, [POINTER(ResidualNorm)]),
+    "equigspr_residual_norm_backward": (ctypes.c_int, [POINTER(ResidualNorm)] + [c_void_p] * 3 + [POINTER(ResidualNormGrads), c_void_p]),
     "equigspr_kabsch_forward": (ctypes.c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p,
                                                c_void_p, c_void_p]),
     "equigspr_kabsch_backward": (ctypes.c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

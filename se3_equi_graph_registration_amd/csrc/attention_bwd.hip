@@ -1,0 +1,379 @@
+// Attention between the points of clouds, backward.  The probabilities are recomputed from the forward's log-sums L:
+//   P = exp2(c S - L),  delta = rowsum(dO * O),  dV = P^T dO,  dP = dO V^T,  dS = P * (dP - delta),  dQ = scale dS K,  dK = scale dS^T Q.
+// Two kernels, seven products: attn_dq_kernel owns 32 packed rows per wave and walks the keys (it also computes delta, once);
+// attn_dkv_kernel owns 32 keys per wave and walks the packed rows -- all query heads of the group, so the gradients of shared keys need
+// no atomics and do not depend on timing.  In each, the score tile is formed with the owned index in the lane, which makes P and dS the
+// B operands of the products that follow as they stand (see attention.hip); the other operand is the staged tile read transposed.
+// P and dS are rounded to the inputs' 16-bit type for those products, everything else is fp32.
+// fp16: dS is about 1/keys of the output gradient and would sink below fp16's range, so it is held as 2^E dS, with E from the largest
+// |dO| and |V| such that the bound |dS| <= 2 dim max|dO| max|V| stays in range; undone in fp32 at the end.
+#include "attention_device.h"
+
+namespace eq {
+
+constexpr int kAmaxBlocks = 256;
+
+template <int T>
+struct AttnBwd {
+    AttnShape s;
+    AttnTensor<T> q, k, v, o, g;              // g: gradient of the output
+    const float* lse;
+    float* delta;                             // [batch, kv_heads, nq * group]
+    float* amax;                              // fp16: [2 * kAmaxBlocks]
+    typename Num<T>::type *gq, *gk, *gv;      // contiguous, each may be null
+    int row_tiles, key_tiles;
+};
+
+// fp16: largest |dO| over the existing rows and |V| over the visible keys, one pair per workgroup
+template <int T>
+__global__ __launch_bounds__(256) void attn_amax_kernel(AttnBwd<T> a) {
+    const AttnShape& s = a.s;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float mg = 0.f, mv = 0.f;
+    const int64_t ng = (int64_t)s.batch * s.nq * s.heads, nv = (int64_t)s.batch * s.nk * s.kv_heads;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < ng; r += kAmaxBlocks * 4) {
+        const int64_t bi = r / s.heads;
+        const int h = (int)(r - bi * s.heads), b = (int)(bi / s.nq), i = (int)(bi - (int64_t)b * s.nq);
+        if (i >= attn_len(s.q_lens, b, s.nq)) continue;
+        const typename Num<T>::type* p = a.g.p + b * a.g.sb + i * a.g.sn + h * a.g.sh;
+        for (int c = lane; c < s.dim; c += 64) mg = fmaxf(mg, fabsf((float)p[c]));
+    }
+    for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < nv; r += kAmaxBlocks * 4) {
+        const int64_t bi = r / s.kv_heads;
+        const int h = (int)(r - bi * s.kv_heads), b = (int)(bi / s.nk), j = (int)(bi - (int64_t)b * s.nk);
+        if (j >= attn_len(s.kv_lens, b, s.nk) || (s.key_mask && !s.key_mask[b * s.mask_stride + j])) continue;
+        const typename Num<T>::type* p = key_row(a.v, b, h, j);
+        for (int c = lane; c < s.dim; c += 64) mv = fmaxf(mv, fabsf((float)p[c]));
+    }
+    __shared__ float part[2][4];
+    for (int o = 32; o; o >>= 1) { mg = fmaxf(mg, __shfl_xor(mg, o)); mv = fmaxf(mv, __shfl_xor(mv, o)); }
+    if (lane == 0) { part[0][wave] = mg; part[1][wave] = mv; }
+    __syncthreads();
+    if (threadIdx.x < 2)
+        a.amax[2 * blockIdx.x + threadIdx.x] = fmaxf(fmaxf(part[threadIdx.x][0], part[threadIdx.x][1]), fmaxf(part[threadIdx.x][2], part[threadIdx.x][3]));
+}
+
+// the power of two dS is held with: 1 except in fp16
+template <int T>
+__device__ __forceinline__ float attn_grad_scale(const AttnBwd<T>& a) {
+    if constexpr (T != kF16) return 1.f;
+    const int lane = threadIdx.x & 63;
+    float mg = 0.f, mv = 0.f;
+#pragma unroll
+    for (int i = 0; i < kAmaxBlocks / 64; ++i) {
+        mg = fmaxf(mg, a.amax[2 * (lane + 64 * i)]);
+        mv = fmaxf(mv, a.amax[2 * (lane + 64 * i) + 1]);
+    }
+    for (int o = 32; o; o >>= 1) { mg = fmaxf(mg, __shfl_xor(mg, o)); mv = fmaxf(mv, __shfl_xor(mv, o)); }
+    const float bound = 2.f * a.s.dim * mg * mv;
+    if (!(bound > 0.f) || bound > 3e38f) return 1.f;
+    const int e = (int)floorf(log2f(60000.f) - log2f(bound));
+    return ldexpf(1.f, e < -60 ? -60 : (e > 60 ? 60 : e));
+}
+
+template <int T, int W, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnBwd<T> a) {
+    constexpr int KT = attn_tile<T, W>(), NT = NW * 64, ROWS = NW * 32, NP = Num<T>::planes;
+    constexpr int KS = W / 16, DB = W / 32, KB = KT / 32;
+    __shared__ __attribute__((aligned(16))) short tile_k[NP * KT * W];
+    __shared__ __attribute__((aligned(16))) short tile_v[NP * KT * W];
+    __shared__ __attribute__((aligned(16))) float hidden[KT];
+    const AttnShape& s = a.s;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int id = xcd_block(blockIdx.x, gridDim.x);
+    const int rt = a.row_tiles - 1 - id % a.row_tiles, bh = id / a.row_tiles, b = bh / s.kv_heads, hk = bh - b * s.kv_heads;
+    const int ql = attn_len(s.q_lens, b, s.nq), kl = attn_len(s.kv_lens, b, s.nk);
+    const int rows = s.nq * s.group, rows_valid = ql * s.group, row0 = rt * ROWS;
+    const int row = row0 + wave * 32 + (lane & 31);
+    const bool ok_row = row < rows_valid;
+    int k_end = kl;
+    const int last_row = min(row0 + ROWS, rows_valid) - 1;
+    if (s.causal && last_row >= 0) k_end = min(k_end, row_point(s, last_row) + kl - ql + 1);
+    if (row0 >= rows_valid || !a.gq) k_end = 0;
+    const int limit = s.causal ? row_point(s, row) + kl - ql : 0x7fffffff;
+    const uint8_t* mask = s.key_mask ? s.key_mask + b * s.mask_stride : nullptr;
+    const int64_t at = (int64_t)bh * rows + row;
+
+    Op8<T> q[KS], g[KS];
+    float delta = 0.f;
+    {
+        const typename Num<T>::type* pq = ok_row ? packed_row(a.q, s, b, hk, row) : nullptr;
+        const typename Num<T>::type* pg = ok_row ? packed_row(a.g, s, b, hk, row) : nullptr;
+        const typename Num<T>::type* po = ok_row ? packed_row(a.o, s, b, hk, row) : nullptr;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int c = ks * 16 + half * 8;
+            q[ks] = planes_of<T>(ok_row ? load8<T>(pq, c, s.dim) : raw_zero<T>());
+            const Raw8<T> rg = ok_row ? load8<T>(pg, c, s.dim) : raw_zero<T>(), ro = ok_row ? load8<T>(po, c, s.dim) : raw_zero<T>();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) delta = fmaf(raw_float<T>(rg, i), raw_float<T>(ro, i), delta);
+            g[ks] = planes_of<T>(rg);
+        }
+    }
+    delta += __shfl_xor(delta, 32);
+    if (row < rows && half == 0) a.delta[at] = delta;
+    if (!a.gq) return;
+    const float lse = ok_row ? a.lse[at] : INFINITY;
+    const float factor = attn_grad_scale<T>(a);
+    pf32x16 acc[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+
+    Stager<T, W, KT, NT> sk, sv;
+    bool vis = false;
+    auto load_tile = [&](int k0) {
+        auto ok = [&](int j) { return k0 + j < k_end && (!mask || mask[k0 + j]); };
+        sk.load([&](int j) { return ok(j) ? key_row(a.k, b, hk, k0 + j) : nullptr; }, s.dim);
+        sv.load([&](int j) { return ok(j) ? key_row(a.v, b, hk, k0 + j) : nullptr; }, s.dim);
+        if (threadIdx.x < KT) vis = ok(threadIdx.x);
+    };
+    if (k_end > 0) load_tile(0);
+    for (int k0 = 0; k0 < k_end; k0 += KT) {
+        __syncthreads();
+        sk.store(tile_k);
+        sv.store(tile_v);
+        if (threadIdx.x < KT) hidden[threadIdx.x] = vis ? 0.f : 1.f;
+        __syncthreads();
+        if (k0 + KT < k_end) load_tile(k0 + KT);
+        const bool edge = mask || k0 + KT > k_end || (s.causal && k0 + KT > row_point(s, row0 + wave * 32) + kl - ql + 1);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            pf32x16 sc, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[r] = dp[r] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                mma<T>(sc, tile_rows<T, W, KT>(tile_k, kb * 32, ks, lane), q[ks]);
+                mma<T>(dp, tile_rows<T, W, KT>(tile_v, kb * 32, ks, lane), g[ks]);
+            }
+            if (edge) {
+#pragma unroll
+                for (int gq = 0; gq < 4; ++gq) {
+                    const int j = kb * 32 + 8 * gq + 4 * half;
+                    const pf32x4 h = *reinterpret_cast<const pf32x4*>(hidden + j);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (h[i] != 0.f || k0 + j + i > limit) sc[4 * gq + i] = -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    x[j] = exp2_fast(fmaf(sc[8 * t + j], s.scale_log2, -lse)) * (dp[8 * t + j] - delta) * factor;
+                const Op8<T> ds = pack8<T>(x);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) mma<T>(acc[d], tile_cols<T, W, KT>(tile_k, kb * 32 + 16 * t, d * 32, lane), ds);
+            }
+        }
+    }
+    if (row >= rows) return;
+    const float back = s.scale / factor;
+    const int i0 = row_point(s, row);
+    typename Num<T>::type* o = a.gq + (((int64_t)b * s.nq + i0) * s.heads + hk * s.group + row - i0 * s.group) * s.dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int gq = 0; gq < 4; ++gq) {
+            const int c = d * 32 + 8 * gq + 4 * half;
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = acc[d][4 * gq + i] * back;
+            store4<T>(o + c, x, s.dim - c);
+        }
+}
+
+template <int T, int W, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnBwd<T> a) {
+    constexpr int RT = attn_tile<T, W>(), NT = NW * 64, KEYS = NW * 32, NP = Num<T>::planes;
+    constexpr int KS = W / 16, DB = W / 32, RB = RT / 32;
+    constexpr float kShift = T == kF16 ? 10.f : 0.f;
+    __shared__ __attribute__((aligned(16))) short tile_q[NP * RT * W];
+    __shared__ __attribute__((aligned(16))) short tile_g[NP * RT * W];
+    __shared__ __attribute__((aligned(16))) float row_lse[RT];
+    __shared__ __attribute__((aligned(16))) float row_delta[RT];
+    __shared__ __attribute__((aligned(16))) int row_limit[RT];
+    const AttnShape& s = a.s;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int id = xcd_block(blockIdx.x, gridDim.x);
+    const int kt = id % a.key_tiles, bh = id / a.key_tiles, b = bh / s.kv_heads, hk = bh - b * s.kv_heads;
+    const int ql = attn_len(s.q_lens, b, s.nq), kl = attn_len(s.kv_lens, b, s.nk);
+    const int rows = s.nq * s.group, rows_valid = ql * s.group, key0 = kt * KEYS;
+    const int key = key0 + wave * 32 + (lane & 31);
+    const bool ok_key = key < kl && (!s.key_mask || s.key_mask[b * s.mask_stride + key]);
+    const int r_end = key0 < kl ? rows_valid : 0;
+    const int r_begin = s.causal ? max(0, key0 - kl + ql) * s.group : 0;      // the first point that sees this tile's first key
+
+    Op8<T> k[KS], v[KS];                      // keys that are not visible: zeros; their lanes' results are replaced at the end
+    {
+        const typename Num<T>::type* pk = ok_key ? key_row(a.k, b, hk, key) : nullptr;
+        const typename Num<T>::type* pv = ok_key ? key_row(a.v, b, hk, key) : nullptr;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int c = ks * 16 + half * 8;
+            k[ks] = planes_of<T>(ok_key ? load8<T>(pk, c, s.dim) : raw_zero<T>());
+            v[ks] = planes_of<T>(ok_key ? load8<T>(pv, c, s.dim) : raw_zero<T>());
+        }
+    }
+    const float factor = attn_grad_scale<T>(a), fs = factor * exp2_fast(-kShift);
+    pf32x16 acc_k[DB], acc_v[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc_k[d][r] = acc_v[d][r] = 0.f;
+
+    Stager<T, W, RT, NT> sq, sg;
+    float my_lse = INFINITY, my_delta = 0.f;
+    int my_limit = -1;
+    auto load_tile = [&](int r0) {
+        sq.load([&](int r) { return r0 + r < r_end ? packed_row(a.q, s, b, hk, r0 + r) : nullptr; }, s.dim);
+        sg.load([&](int r) { return r0 + r < r_end ? packed_row(a.g, s, b, hk, r0 + r) : nullptr; }, s.dim);
+        if (threadIdx.x < RT) {
+            const int r = r0 + threadIdx.x;
+            const int64_t at = (int64_t)bh * rows + r;
+            my_lse = r < r_end ? a.lse[at] : INFINITY;
+            my_delta = r < r_end ? a.delta[at] : 0.f;
+            my_limit = row_point(s, r) + kl - ql;
+        }
+    };
+    if (r_begin < r_end) load_tile(r_begin);
+    for (int r0 = r_begin; r0 < r_end; r0 += RT) {
+        __syncthreads();
+        sq.store(tile_q);
+        sg.store(tile_g);
+        if (threadIdx.x < RT) { row_lse[threadIdx.x] = kShift - my_lse; row_delta[threadIdx.x] = my_delta; row_limit[threadIdx.x] = my_limit; }
+        __syncthreads();
+        if (r0 + RT < r_end) load_tile(r0 + RT);
+        const bool edge = s.causal && key0 + wave * 32 + 31 > row_point(s, r0) + kl - ql;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            pf32x16 sc, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[r] = dp[r] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                mma<T>(sc, tile_rows<T, W, RT>(tile_q, rb * 32, ks, lane), k[ks]);
+                mma<T>(dp, tile_rows<T, W, RT>(tile_g, rb * 32, ks, lane), v[ks]);
+            }
+#pragma unroll
+            for (int gr = 0; gr < 4; ++gr) {
+                const int r = rb * 32 + 8 * gr + 4 * half;
+                const pf32x4 sub = *reinterpret_cast<const pf32x4*>(row_lse + r), del = *reinterpret_cast<const pf32x4*>(row_delta + r);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = exp2_fast(fmaf(sc[4 * gr + i], s.scale_log2, sub[i]));
+                    sc[4 * gr + i] = p;
+                    dp[4 * gr + i] = p * (dp[4 * gr + i] - del[i]) * fs;
+                }
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (key > row_limit[r + i]) sc[4 * gr + i] = dp[4 * gr + i] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                float x[8], y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { x[j] = sc[8 * t + j]; y[j] = dp[8 * t + j]; }
+                const Op8<T> p = pack8<T>(x), ds = pack8<T>(y);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    mma<T>(acc_v[d], tile_cols<T, W, RT>(tile_g, rb * 32 + 16 * t, d * 32, lane), p);
+                    mma<T>(acc_k[d], tile_cols<T, W, RT>(tile_q, rb * 32 + 16 * t, d * 32, lane), ds);
+                }
+            }
+        }
+    }
+    if (key >= s.nk) return;
+    const float back_k = s.scale / factor, back_v = exp2_fast(-kShift);
+    const int64_t o = (((int64_t)b * s.nk + key) * s.kv_heads + hk) * s.dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int gr = 0; gr < 4; ++gr) {
+            const int c = d * 32 + 8 * gr + 4 * half;
+            float x[4], y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = ok_key ? acc_k[d][4 * gr + i] * back_k : 0.f;
+                y[i] = ok_key ? acc_v[d][4 * gr + i] * back_v : 0.f;
+            }
+            if (a.gk) store4<T>(a.gk + o + c, x, s.dim - c);
+            if (a.gv) store4<T>(a.gv + o + c, y, s.dim - c);
+        }
+}
+
+// Four waves share a tile when that still gives every compute unit a workgroup; one wave otherwise (shorter runs, more of them).
+static int attn_bwd_waves(int64_t owned, int64_t heads) { return ceil_div(owned, 128) * heads >= 256 ? 4 : 1; }
+
+template <int T, int W>
+static int attn_bwd_launch(AttnBwd<T>& a, hipStream_t st) {
+    const AttnShape& s = a.s;
+    const int64_t heads = (int64_t)s.batch * s.kv_heads;
+    const int wq = attn_bwd_waves((int64_t)s.nq * s.group, heads), wk = attn_bwd_waves(s.nk, heads);
+    a.row_tiles = ceil_div((int64_t)s.nq * s.group, 32 * wq);
+    a.key_tiles = ceil_div(s.nk, 32 * wk);
+    const int64_t bq = a.row_tiles * heads, bk = a.key_tiles * heads;
+    EQ_CHECK_ARG(bq < (1 << 24) && bk < (1 << 24), EQUIGSPR_ENOTSUP, "attention_backward: more workgroups than one launch takes");
+    if (T == kF16) {
+        attn_amax_kernel<T><<<kAmaxBlocks, 256, 0, st>>>(a);
+        EQ_CHECK_LAUNCH("attention_backward (range)");
+    }
+    if (bq) {
+        if (wq == 1) attn_dq_kernel<T, W, 1><<<(unsigned)bq, 64, 0, st>>>(a);
+        else attn_dq_kernel<T, W, 4><<<(unsigned)bq, 256, 0, st>>>(a);
+        EQ_CHECK_LAUNCH("attention_backward (rows)");
+    }
+    if (bk && (a.gk || a.gv)) {
+        if (wk == 1) attn_dkv_kernel<T, W, 1><<<(unsigned)bk, 64, 0, st>>>(a);
+        else attn_dkv_kernel<T, W, 4><<<(unsigned)bk, 256, 0, st>>>(a);
+        EQ_CHECK_LAUNCH("attention_backward (keys)");
+    }
+    return 0;
+}
+
+template <int T>
+static int attn_bwd(const equigspr_attention* d, const AttnShape& s, const void* out, const float* lse, const equigspr_attention_tensor* grad_out,
+                    float* work, void* gq, void* gk, void* gv, hipStream_t st) {
+    using E = typename Num<T>::type;
+    AttnBwd<T> a;
+    a.s = s;
+    a.q = attn_tensor<T>(d->q, s.dim);
+    a.k = attn_tensor<T>(d->k, s.dim);
+    a.v = attn_tensor<T>(d->v, s.dim);
+    a.g = attn_tensor<T>(*grad_out, s.dim);
+    const equigspr_attention_tensor o = {const_cast<void*>(out), (int64_t)s.nq * s.heads * s.dim, (int64_t)s.heads * s.dim, s.dim};
+    a.o = attn_tensor<T>(o, s.dim);
+    a.lse = lse;
+    a.amax = work;
+    a.delta = work + 2 * kAmaxBlocks;
+    a.gq = (E*)gq; a.gk = (E*)gk; a.gv = (E*)gv;
+    return s.dim <= 32 ? attn_bwd_launch<T, 32>(a, st) : s.dim <= 64 ? attn_bwd_launch<T, 64>(a, st) : attn_bwd_launch<T, 128>(a, st);
+}
+
+}  // namespace eq
+
+extern "C" int64_t equigspr_attention_backward_work_size(const equigspr_attention* d) {
+    eq::AttnShape s;
+    if (eq::attn_shape(d, &s) != 0) return -1;
+    return 2 * eq::kAmaxBlocks + (int64_t)s.batch * s.kv_heads * s.nq * s.group;
+}
+
+extern "C" int equigspr_attention_backward(const equigspr_attention* d, const void* out, const float* lse, const equigspr_attention_tensor* grad_out,
+                                           float* work, void* grad_q, void* grad_k, void* grad_v, void* stream) {
+    eq::AttnShape s;
+    if (const int rc = eq::attn_shape(d, &s)) return rc;
+    EQ_CHECK_ARG(grad_out && work, EQUIGSPR_EINVAL, "attention_backward: grad_out or work is null");
+    EQ_CHECK_ARG(!s.batch || !s.nq || (out && lse && grad_out->data), EQUIGSPR_EINVAL, "attention_backward: out, lse or grad_out is null");
+    if (s.batch == 0) return 0;
+    hipStream_t st = (hipStream_t)stream;
+    switch (d->dtype) {
+        case EQUIGSPR_F32: return eq::attn_bwd<eq::kF32>(d, s, out, lse, grad_out, work, grad_q, grad_k, grad_v, st);
+        case EQUIGSPR_BF16: return eq::attn_bwd<eq::kBF16>(d, s, out, lse, grad_out, work, grad_q, grad_k, grad_v, st);
+        default: return eq::attn_bwd<eq::kF16>(d, s, out, lse, grad_out, work, grad_q, grad_k, grad_v, st);
+    }
+}

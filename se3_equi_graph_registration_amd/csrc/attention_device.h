@@ -1,0 +1,118 @@
+// What the attention kernels (attention.hip, attention_bwd.hip) share: the problem's description, the packed row order, the staging
+// of rows into LDS tiles.
+//
+// Rows are PACKED: the G = heads / kv_heads query heads that share a key head form one row axis, row r = i G + g of point i and head
+// g of the group.  A key tile is then read once for the whole group, and the gradients of the shared keys are summed inside one
+// workgroup, in a fixed order.
+#pragma once
+#include "planes.h"
+
+namespace eq {
+
+struct AttnShape {
+    int batch, nq, nk, heads, kv_heads, group, dim;
+    unsigned group_magic;                     // ceil(2^32 / group): r / group = umulhi(r, magic) while rows * group < 2^32 (host check)
+    float scale_log2;                         // scale * log2(e)
+    float scale;
+    int causal;
+    const int32_t* q_lens;                    // [batch] or null
+    const int32_t* kv_lens;
+    const uint8_t* key_mask;                  // [batch, nk] or null, non-zero = visible
+    int64_t mask_stride;
+};
+
+// [batch, points, heads, dim] with unit stride in dim
+template <int T>
+struct AttnTensor {
+    typename Num<T>::type* p;
+    int64_t sb, sn, sh;
+};
+
+__device__ __forceinline__ int attn_len(const int32_t* lens, int b, int n) {
+    if (!lens) return n;
+    const int v = lens[b];
+    return v < 0 ? 0 : (v > n ? n : v);
+}
+__device__ __forceinline__ int row_point(const AttnShape& s, int r) { return s.group == 1 ? r : (int)__umulhi((unsigned)r, s.group_magic); }
+
+template <int T>
+__device__ __forceinline__ typename Num<T>::type* packed_row(const AttnTensor<T>& t, const AttnShape& s, int b, int hk, int r) {
+    const int i = row_point(s, r), g = r - i * s.group;
+    return t.p + b * t.sb + i * t.sn + (int64_t)(hk * s.group + g) * t.sh;
+}
+template <int T>
+__device__ __forceinline__ typename Num<T>::type* key_row(const AttnTensor<T>& t, int b, int hk, int j) {
+    return t.p + b * t.sb + j * t.sn + (int64_t)hk * t.sh;
+}
+
+// ROWS x W values from memory to the planes of a tile by NT threads: load() to registers, store() to LDS, so that the next tile's
+// loads are in flight under this tile's products
+template <int T, int W, int ROWS, int NT>
+struct Stager {
+    static constexpr int kChunks = W / 8, kPer = ROWS * kChunks / NT, kPlane = ROWS * W;      // chunks of a row, of a thread; values of a plane
+    static_assert(kPer * NT == ROWS * kChunks, "whole chunks per thread");
+    Raw8<T> raw[kPer];
+    // row_of(r) -> pointer of row r, or null for a row of zeros
+    template <class F>
+    __device__ __forceinline__ void load(F row_of, int width) {
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+            const int id = threadIdx.x + u * NT;
+            const typename Num<T>::type* row = row_of(id / kChunks);
+            raw[u] = row ? load8<T>(row, (id % kChunks) * 8, width) : raw_zero<T>();
+        }
+    }
+    __device__ __forceinline__ void store(short* tile) const {
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+            const int id = threadIdx.x + u * NT;
+            const Op8<T> o = planes_of<T>(raw[u]);
+#pragma unroll
+            for (int p = 0; p < Num<T>::planes; ++p)
+                *reinterpret_cast<s16x8*>(tile + p * kPlane + Tile<W>::at(id / kChunks, id % kChunks)) = o.p[p];
+        }
+    }
+};
+
+// A operand: 32 rows of the tile from row0, k-step ks (16 columns)
+template <int T, int W, int ROWS>
+__device__ __forceinline__ Op8<T> tile_rows(const short* tile, int row0, int ks, int lane) {
+    Op8<T> o;
+#pragma unroll
+    for (int p = 0; p < Num<T>::planes; ++p) o.p[p] = Tile<W>::row8(tile + p * ROWS * W, row0 + (lane & 31), 2 * ks + (lane >> 5));
+    return o;
+}
+// A operand of the transposed tile: 32 columns from col0 as rows; the contraction runs over the 16 tile rows from row0 in the order in
+// which the C tile of an earlier product holds them (slot j of half h is row 8 (j >> 2) + 4 h + (j & 3)), so that product's result is
+// the B operand as it stands
+template <int T, int W, int ROWS>
+__device__ __forceinline__ Op8<T> tile_cols(const short* tile, int row0, int col0, int lane) {
+    Op8<T> o;
+    const int r = row0 + 4 * (lane >> 5), c = col0 + (lane & 16);
+#pragma unroll
+    for (int p = 0; p < Num<T>::planes; ++p)
+        o.p[p] = join8(Tile<W>::col4(tile + p * ROWS * W, r, c, lane), Tile<W>::col4(tile + p * ROWS * W, r + 8, c, lane));
+    return o;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+constexpr int kAttnMaxDim = 128;
+
+// rows of a staged tile: 64, except where three planes of a wide head would take too much LDS
+template <int T, int W> constexpr int attn_tile() { return T == kF32 && W > 32 ? 32 : 64; }
+
+// ---- host side
+template <int T>
+static inline AttnTensor<T> attn_tensor(const equigspr_attention_tensor& t, int dim) {
+    using E = typename Num<T>::type;
+    AttnTensor<T> r;
+    r.p = (E*)t.data;
+    r.sb = t.stride_batch; r.sn = t.stride_point; r.sh = t.stride_head;
+    return r;
+}
+
+// checks the description and derives what the kernels use; 0 or an error code
+int attn_shape(const equigspr_attention* d, AttnShape* s);
+
+}  // namespace eq

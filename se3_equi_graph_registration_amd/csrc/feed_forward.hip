@@ -1,0 +1,432 @@
+// The gated feed-forward block:  z = x Wg^T + bg,  u = x Wu^T + bu,  h = act(z) * u,  y = h Wd^T + bd,  and its backward
+//   dh = dy Wd,  dz = dh u act'(z),  du = dh act(z),  dx = dz Wg + du Wu,  dWg = dz^T x,  dWu = du^T x,  dWd = dy^T h,  biases: column sums.
+// One matrix-product kernel, three epilogues:
+//   kGate   both projections of a tile from one staged x tile, activation and product in registers: h (and, for training, z | u) leave once
+//   kGrad   dh of a tile never leaves: the epilogue reads z | u and writes dz | du and h
+//   kPlain  C = A B^T (+ bias), or fp32 partial tiles of a cut contraction, summed in order by ff_sum_kernel
+// z | u and dz | du are [rows, 2 hidden]: dx is ONE product over 2 hidden, dWg and dWu are the two halves of ONE product's rows.
+// A product's operands may run along or across the contraction in memory; across, the tile is read transposed (planes.h), so nothing
+// is ever transposed in memory.  Products accumulate in fp32; h, z, u, dz, du are stored in the inputs' type (what a 16-bit program
+// keeps between its layers: one rounding each), fp32 inputs stay fp32 with three-plane products.
+// Bound: the matrix pipe for many rows, the weights' bytes for few.
+#include "planes.h"
+
+namespace eq {
+
+enum { kPlain = 0, kGate = 1, kGrad = 2 };
+enum { kSilu = EQUIGSPR_ACT_SILU, kGelu = EQUIGSPR_ACT_GELU, kRelu = EQUIGSPR_ACT_RELU };
+
+// one operand as rows of `len` values; row r lies at p + r * ld, rows at or behind `split` in q (two matrices that act as one)
+template <int T>
+struct FfOperand {
+    const typename Num<T>::type *p, *q;
+    int64_t ld;
+    int rows, split, len;
+    __device__ __forceinline__ const typename Num<T>::type* row(int r) const { return r < split ? p + r * ld : q + (r - split) * ld; }
+};
+
+template <int T>
+struct FfArgs {
+    using E = typename Num<T>::type;
+    FfOperand<T> a, b;                        // the output's rows and columns
+    int m, n, k;                              // kGate: n counts the columns of one projection
+    int tiles_m, tiles_n, cuts, cut_k;        // cut_k: contraction length of a cut (a multiple of the k tile)
+    E* c;                                     // [m, n]
+    const E *bias, *bias2;
+    float* part;                              // [cuts][m][n]
+    E* zu;                                    // kGate: written if not null; kGrad: read.  [m, 2 n]
+    E* dzu;                                   // kGrad: [m, 2 n]
+    E* h;                                     // kGrad: [m, n]
+    int act;
+};
+
+// act(z) and its derivative
+__device__ __forceinline__ void activate(int act, float z, float& a, float& d) {
+    if (act == kSilu) {
+        const float s = 1.f / (1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
+        a = z * s;
+        d = s * (1.f + z * (1.f - s));
+    } else if (act == kGelu) {
+        const float c = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+        a = z * c;
+        d = fmaf(z * 0.39894228040143268f, __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z), c);
+    } else {
+        a = fmaxf(z, 0.f);
+        d = z > 0.f ? 1.f : 0.f;
+    }
+}
+
+// tile of 128 x 128 outputs, four waves of 64 x 64
+constexpr int kFfTile = 128;
+template <int T> constexpr int ff_k_tile() { return T == kF32 ? 32 : 64; }
+
+// kAcross: the operand's contraction runs across its rows in memory (tile [k][m]) instead of along them (tile [m][k])
+template <int T, bool kAcross>
+struct FfTile {
+    static constexpr int BK = ff_k_tile<T>(), W = kAcross ? kFfTile : BK, ROWS = kAcross ? BK : kFfTile;
+    static constexpr int kPlane = W * ROWS, kPer = ROWS * W / 8 / 256;
+    Raw8<T> raw[kPer];
+    // outer0: first output row / column of the tile; k0: first contraction index; k_end bounds it
+    template <class F>
+    __device__ __forceinline__ void load(const FfOperand<T>& o, int outer0, int k0, int k_end, F outer_row) {
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+            const int id = threadIdx.x + u * 256, r = id / (W / 8), c = id % (W / 8) * 8;
+            if constexpr (kAcross) {
+                raw[u] = k0 + r < k_end ? load8<T>(o.row(k0 + r) + outer0, c, o.len - outer0) : raw_zero<T>();
+            } else {
+                const typename Num<T>::type* row = outer_row(r);
+                raw[u] = row ? load8<T>(row + k0, c, k_end - k0) : raw_zero<T>();
+            }
+        }
+    }
+    __device__ __forceinline__ void store(short* tile) const {
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+            const int id = threadIdx.x + u * 256;
+            const Op8<T> o = planes_of<T>(raw[u]);
+#pragma unroll
+            for (int p = 0; p < Num<T>::planes; ++p) *reinterpret_cast<s16x8*>(tile + p * kPlane + Tile<W>::at(id / (W / 8), id % (W / 8))) = o.p[p];
+        }
+    }
+    // 32 outputs from o0, k-step ks
+    __device__ static __forceinline__ Op8<T> operand(const short* tile, int o0, int ks, int lane) {
+        Op8<T> r;
+#pragma unroll
+        for (int p = 0; p < Num<T>::planes; ++p) {
+            const short* t = tile + p * kPlane;
+            if constexpr (kAcross) {
+                const int k = 16 * ks + 8 * (lane >> 5), c = o0 + (lane & 16);
+                r.p[p] = join8(Tile<W>::col4(t, k, c, lane), Tile<W>::col4(t, k + 4, c, lane));
+            } else {
+                r.p[p] = Tile<W>::row8(t, o0 + (lane & 31), 2 * ks + (lane >> 5));
+            }
+        }
+        return r;
+    }
+};
+
+template <int T, bool kAcrossA, bool kAcrossB, int kEpi>
+__global__ __launch_bounds__(256) void ff_product_kernel(FfArgs<T> g) {
+    using TA = FfTile<T, kAcrossA>;
+    using TB = FfTile<T, kAcrossB>;
+    constexpr int BK = ff_k_tile<T>(), NP = Num<T>::planes, TN = kEpi == kGate ? kFfTile / 2 : kFfTile;
+    __shared__ __attribute__((aligned(16))) short tile_a[NP * TA::kPlane];
+    __shared__ __attribute__((aligned(16))) short tile_b[NP * TB::kPlane];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wm = wave >> 1, wn = wave & 1;
+    int id = xcd_block(blockIdx.x, gridDim.x);
+    const int tm = id % g.tiles_m;
+    id /= g.tiles_m;
+    const int tn = id % g.tiles_n, cut = id / g.tiles_n;
+    const int m0 = tm * kFfTile, n0 = tn * TN, k_begin = cut * g.cut_k, k_end = min(g.k, k_begin + g.cut_k);
+    auto row_a = [&](int r) { return m0 + r < g.a.rows ? g.a.row(m0 + r) : nullptr; };
+    auto row_b = [&](int r) -> const typename Num<T>::type* {
+        if constexpr (kEpi == kGate) {            // tile rows 0..63: gate columns, 64..127: the same columns of the other projection
+            const int c = n0 + (r & 63);
+            return c < g.n ? (r < 64 ? g.b.p : g.b.q) + c * g.b.ld : nullptr;
+        } else {
+            return n0 + r < g.b.rows ? g.b.row(n0 + r) : nullptr;
+        }
+    };
+    // acc[i][j]: C tile with the output's columns in the registers (block j) and its rows in the lanes (block i)
+    pf32x16 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    const int om[2] = {wm * 64, wm * 64 + 32};
+    const int on[2] = {kEpi == kGate ? wn * 32 : wn * 64, kEpi == kGate ? 64 + wn * 32 : wn * 64 + 32};
+    TA sa;
+    TB sb;
+    sa.load(g.a, m0, k_begin, k_end, row_a);
+    sb.load(g.b, n0, k_begin, k_end, row_b);
+    for (int k0 = k_begin; k0 < k_end; k0 += BK) {
+        __syncthreads();
+        sa.store(tile_a);
+        sb.store(tile_b);
+        __syncthreads();
+        if (k0 + BK < k_end) {
+            sa.load(g.a, m0, k0 + BK, k_end, row_a);
+            sb.load(g.b, n0, k0 + BK, k_end, row_b);
+        }
+#pragma unroll
+        for (int ks = 0; ks < BK / 16; ++ks) {
+            Op8<T> pa[2], pb[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                pa[i] = TA::operand(tile_a, om[i], ks, lane);
+                pb[i] = TB::operand(tile_b, on[i], ks, lane);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma<T>(acc[i][j], pb[j], pa[i]);
+        }
+    }
+    using E = typename Num<T>::type;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = m0 + om[i] + (lane & 31);
+        if (row >= g.m) continue;
+        if constexpr (kEpi == kGate) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int col = n0 + on[0] + 8 * q + 4 * half, left = g.n - col;
+                if (left <= 0) continue;
+                float z[4], u[4], h[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    z[e] = acc[i][0][4 * q + e] + (g.bias && e < left ? (float)g.bias[col + e] : 0.f);
+                    u[e] = acc[i][1][4 * q + e] + (g.bias2 && e < left ? (float)g.bias2[col + e] : 0.f);
+                    float a, d;
+                    activate(g.act, z[e], a, d);
+                    h[e] = a * u[e];
+                }
+                store4<T>(g.c + (int64_t)row * g.n + col, h, left);
+                if (g.zu) {
+                    store4<T>(g.zu + (int64_t)row * 2 * g.n + col, z, left);
+                    store4<T>(g.zu + (int64_t)row * 2 * g.n + g.n + col, u, left);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int col = n0 + on[j] + 8 * q + 4 * half, left = g.n - col;
+                    if (left <= 0) continue;
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
+                    if constexpr (kEpi == kGrad) {
+                        const E* pz = g.zu + (int64_t)row * 2 * g.n + col;
+                        float dz[4], du[4], h[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float z = e < left ? (float)pz[e] : 0.f, u = e < left ? (float)pz[g.n + e] : 0.f;
+                            float a, d;
+                            activate(g.act, z, a, d);
+                            h[e] = a * u;
+                            dz[e] = v[e] * u * d;
+                            du[e] = v[e] * a;
+                        }
+                        store4<T>(g.dzu + (int64_t)row * 2 * g.n + col, dz, left);
+                        store4<T>(g.dzu + (int64_t)row * 2 * g.n + g.n + col, du, left);
+                        store4<T>(g.h + (int64_t)row * g.n + col, h, left);
+                    } else if (g.cuts > 1) {
+                        store4<kF32>(g.part + ((int64_t)cut * g.m + row) * g.n + col, v, left);
+                    } else {
+                        if (g.bias)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[e] += e < left ? (float)g.bias[col + e] : 0.f;
+                        store4<T>(g.c + (int64_t)row * g.n + col, v, left);
+                    }
+                }
+        }
+    }
+}
+
+// the parts of a cut contraction, in order
+template <int T>
+__global__ __launch_bounds__(256) void ff_sum_kernel(FfArgs<T> g) {
+    const int64_t n = (int64_t)g.m * g.n;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        float v = g.bias ? (float)g.bias[i % g.n] : 0.f;
+        for (int c = 0; c < g.cuts; ++c) v += g.part[c * n + i];
+        store_value<T>(g.c + i, v);
+    }
+}
+
+// column sums of [rows, width] (the biases' gradients): runs of rows, then the runs in order
+template <int T>
+__global__ __launch_bounds__(256) void ff_columns_kernel(const typename Num<T>::type* x, int rows, int width, int run, float* part) {
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6, r0 = blockIdx.y * run, r1 = min(rows, r0 + run);
+    __shared__ float lds[4][64];
+    float v = 0.f;
+    if (c < width)
+        for (int r = r0 + q; r < r1; r += 4) v += (float)x[(int64_t)r * width + c];
+    lds[q][threadIdx.x & 63] = v;
+    __syncthreads();
+    if (q == 0 && c < width) part[(int64_t)blockIdx.y * width + c] = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
+}
+template <int T>
+__global__ __launch_bounds__(256) void ff_columns_sum_kernel(const float* part, int runs, int width, typename Num<T>::type* out) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= width) return;
+    float v = 0.f;
+    for (int r = 0; r < runs; ++r) v += part[(int64_t)r * width + c];
+    store_value<T>(out + c, v);
+}
+
+struct FfShape { int rows, width, hidden, out; };
+
+// Cuts of a contraction: when the output's tiles leave compute units idle, into parts of at least four k tiles.
+static int ff_cuts(int64_t tiles, int k, int bk) {
+    if (tiles >= 256) return 1;
+    const int64_t most = k / (4 * bk), want = 512 / (tiles > 0 ? tiles : 1);
+    const int64_t c = want < most ? want : most;
+    return c > 1 ? (int)c : 1;
+}
+static int64_t ff_part_size(int m, int n, int k, int bk) {
+    const int64_t c = ff_cuts((int64_t)ceil_div(m, kFfTile) * ceil_div(n, kFfTile), k, bk);
+    return c > 1 ? c * m * n : 0;
+}
+constexpr int kFfRun = 256;                   // rows of a run of a column sum
+
+template <int T, bool kAcrossA, bool kAcrossB, int kEpi>
+static int ff_product(FfArgs<T> g, hipStream_t st, const char* what) {
+    constexpr int BK = ff_k_tile<T>(), TN = kEpi == kGate ? kFfTile / 2 : kFfTile;
+    g.tiles_m = ceil_div(g.m, kFfTile);
+    g.tiles_n = ceil_div(g.n, TN);
+    g.cuts = kEpi == kPlain ? ff_cuts((int64_t)g.tiles_m * g.tiles_n, g.k, BK) : 1;
+    g.cut_k = ceil_div(ceil_div(g.k, g.cuts), BK) * BK;
+    g.cuts = ceil_div(g.k, g.cut_k);
+    const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.cuts;
+    if (blocks == 0) return 0;
+    EQ_CHECK_ARG(blocks < (1 << 24), EQUIGSPR_ENOTSUP, "%s: more workgroups than one launch takes", what);
+    ff_product_kernel<T, kAcrossA, kAcrossB, kEpi><<<(unsigned)blocks, 256, 0, st>>>(g);
+    EQ_CHECK_LAUNCH(what);
+    if (g.cuts > 1) {
+        const int64_t n = ceil_div((int64_t)g.m * g.n, 256);
+        ff_sum_kernel<T><<<(unsigned)(n < 4096 ? n : 4096), 256, 0, st>>>(g);
+        EQ_CHECK_LAUNCH(what);
+    }
+    return 0;
+}
+
+template <int T>
+static FfOperand<T> ff_operand(const void* p, int rows, int len) {
+    using E = typename Num<T>::type;
+    return {(const E*)p, (const E*)p, len, rows, rows, len};
+}
+
+template <int T>
+static int ff_forward(const equigspr_gated_feed_forward* d, void* y, void* h, void* zu, float* work, hipStream_t st) {
+    using E = typename Num<T>::type;
+    FfArgs<T> g = {};
+    g.act = d->activation;
+    g.a = ff_operand<T>(d->x, d->rows, d->width);
+    g.b = ff_operand<T>(d->w_gate, d->hidden, d->width);
+    g.b.q = (const E*)d->w_up;
+    g.m = d->rows; g.n = d->hidden; g.k = d->width;
+    g.bias = (const E*)d->b_gate; g.bias2 = (const E*)d->b_up;
+    g.c = (E*)h; g.zu = (E*)zu;
+    if (const int rc = ff_product<T, false, false, kGate>(g, st, "gated_feed_forward (projections)")) return rc;
+    g.a = ff_operand<T>(h, d->rows, d->hidden);
+    g.b = ff_operand<T>(d->w_down, d->out, d->hidden);
+    g.n = d->out; g.k = d->hidden;
+    g.bias = (const E*)d->b_down; g.bias2 = nullptr;
+    g.c = (E*)y; g.zu = nullptr; g.part = work;
+    return ff_product<T, false, false, kPlain>(g, st, "gated_feed_forward (output)");
+}
+
+template <int T>
+static int ff_column_sum(const void* x, int rows, int width, float* work, void* out, hipStream_t st) {
+    using E = typename Num<T>::type;
+    const int runs = ceil_div(rows, kFfRun);
+    ff_columns_kernel<T><<<dim3(ceil_div(width, 64), runs), 256, 0, st>>>((const E*)x, rows, width, kFfRun, work);
+    EQ_CHECK_LAUNCH("gated_feed_forward_backward (biases)");
+    ff_columns_sum_kernel<T><<<ceil_div(width, 256), 256, 0, st>>>(work, runs, width, (E*)out);
+    EQ_CHECK_LAUNCH("gated_feed_forward_backward (biases)");
+    return 0;
+}
+
+template <int T>
+static int ff_backward(const equigspr_gated_feed_forward* d, const void* gy, const void* zu, void* h, void* dzu, float* work,
+                       const equigspr_gated_feed_forward_grads* o, hipStream_t st) {
+    using E = typename Num<T>::type;
+    const int r = d->rows, w = d->width, hd = d->hidden, out = d->out;
+    FfArgs<T> g = {};
+    g.act = d->activation;
+    // dh = dy Wd: rows of dy along the contraction (out), Wd [out, hidden] across it
+    g.a = ff_operand<T>(gy, r, out);
+    g.b = ff_operand<T>(d->w_down, out, hd);
+    g.m = r; g.n = hd; g.k = out;
+    g.zu = (E*)const_cast<void*>(zu); g.dzu = (E*)dzu; g.h = (E*)h;
+    if (const int rc = ff_product<T, false, true, kGrad>(g, st, "gated_feed_forward_backward (hidden)")) return rc;
+    g.zu = g.dzu = g.h = nullptr;
+    g.part = work;
+    if (o->grad_x) {                          // [dz | du] [Wg ; Wu]
+        g.a = ff_operand<T>(dzu, r, 2 * hd);
+        g.b = ff_operand<T>(d->w_gate, 2 * hd, w);
+        g.b.split = hd;
+        g.b.q = (const E*)d->w_up;
+        g.m = r; g.n = w; g.k = 2 * hd;
+        g.c = (E*)o->grad_x;
+        if (const int rc = ff_product<T, false, true, kPlain>(g, st, "gated_feed_forward_backward (input)")) return rc;
+    }
+    if (o->grad_w_gate_up) {                  // [dz | du]^T x
+        g.a = ff_operand<T>(dzu, r, 2 * hd);
+        g.b = ff_operand<T>(d->x, r, w);
+        g.m = 2 * hd; g.n = w; g.k = r;
+        g.c = (E*)o->grad_w_gate_up;
+        if (const int rc = ff_product<T, true, true, kPlain>(g, st, "gated_feed_forward_backward (projections)")) return rc;
+    }
+    if (o->grad_w_down) {                     // dy^T h
+        g.a = ff_operand<T>(gy, r, out);
+        g.b = ff_operand<T>(h, r, hd);
+        g.m = out; g.n = hd; g.k = r;
+        g.c = (E*)o->grad_w_down;
+        if (const int rc = ff_product<T, true, true, kPlain>(g, st, "gated_feed_forward_backward (output)")) return rc;
+    }
+    if (o->grad_b_gate_up)
+        if (const int rc = ff_column_sum<T>(dzu, r, 2 * hd, work, o->grad_b_gate_up, st)) return rc;
+    if (o->grad_b_down)
+        if (const int rc = ff_column_sum<T>(gy, r, out, work, o->grad_b_down, st)) return rc;
+    return 0;
+}
+
+static int ff_check(const equigspr_gated_feed_forward* d) {
+    EQ_CHECK_ARG(d, EQUIGSPR_EINVAL, "gated_feed_forward: null description");
+    EQ_CHECK_ARG(d->dtype == EQUIGSPR_F32 || d->dtype == EQUIGSPR_BF16 || d->dtype == EQUIGSPR_F16, EQUIGSPR_EINVAL, "gated_feed_forward: unknown dtype %d", d->dtype);
+    EQ_CHECK_ARG(d->activation == kSilu || d->activation == kGelu || d->activation == kRelu, EQUIGSPR_EINVAL, "gated_feed_forward: unknown activation %d", d->activation);
+    EQ_CHECK_ARG(d->rows >= 0 && d->width >= 1 && d->hidden >= 1 && d->out >= 1, EQUIGSPR_EINVAL, "gated_feed_forward: bad sizes");
+    EQ_CHECK_ARG(d->rows < (1 << 23) && d->width < (1 << 20) && d->hidden < (1 << 20) && d->out < (1 << 20), EQUIGSPR_ENOTSUP, "gated_feed_forward: sizes beyond the kernels' range");
+    EQ_CHECK_ARG(d->w_gate && d->w_up && d->w_down && (d->x || !d->rows), EQUIGSPR_EINVAL, "gated_feed_forward: null tensor");
+    return 0;
+}
+
+}  // namespace eq
+
+extern "C" int64_t equigspr_gated_feed_forward_work_size(const equigspr_gated_feed_forward* d) {
+    if (eq::ff_check(d) != 0) return -1;
+    return eq::ff_part_size(d->rows, d->out, d->hidden, d->dtype == EQUIGSPR_F32 ? eq::ff_k_tile<eq::kF32>() : eq::ff_k_tile<eq::kBF16>());
+}
+
+extern "C" int equigspr_gated_feed_forward_forward(const equigspr_gated_feed_forward* d, void* y, void* h, void* zu, float* work, void* stream) {
+    if (const int rc = eq::ff_check(d)) return rc;
+    if (d->rows == 0) return 0;
+    EQ_CHECK_ARG(y && h && (work || equigspr_gated_feed_forward_work_size(d) == 0), EQUIGSPR_EINVAL, "gated_feed_forward_forward: null output or work");
+    hipStream_t st = (hipStream_t)stream;
+    switch (d->dtype) {
+        case EQUIGSPR_F32: return eq::ff_forward<eq::kF32>(d, y, h, zu, work, st);
+        case EQUIGSPR_BF16: return eq::ff_forward<eq::kBF16>(d, y, h, zu, work, st);
+        default: return eq::ff_forward<eq::kF16>(d, y, h, zu, work, st);
+    }
+}
+
+extern "C" int64_t equigspr_gated_feed_forward_backward_work_size(const equigspr_gated_feed_forward* d) {
+    if (eq::ff_check(d) != 0) return -1;
+    const int bk = d->dtype == EQUIGSPR_F32 ? eq::ff_k_tile<eq::kF32>() : eq::ff_k_tile<eq::kBF16>();
+    int64_t n = eq::ff_part_size(d->rows, d->width, 2 * d->hidden, bk);
+    const int64_t up = eq::ff_part_size(2 * d->hidden, d->width, d->rows, bk), down = eq::ff_part_size(d->out, d->hidden, d->rows, bk);
+    const int64_t widest = 2 * d->hidden > d->out ? 2 * d->hidden : d->out, sums = (int64_t)eq::ceil_div(d->rows, eq::kFfRun) * widest;
+    n = up > n ? up : n;
+    n = down > n ? down : n;
+    return sums > n ? sums : n;
+}
+
+extern "C" int equigspr_gated_feed_forward_backward(const equigspr_gated_feed_forward* d, const void* grad_y, const void* zu, void* h, void* dzu, float* work,
+                                                    const equigspr_gated_feed_forward_grads* grads, void* stream) {
+    if (const int rc = eq::ff_check(d)) return rc;
+    if (d->rows == 0) return 0;
+    EQ_CHECK_ARG(grad_y && zu && h && dzu && work && grads, EQUIGSPR_EINVAL, "gated_feed_forward_backward: null tensor");
+    hipStream_t st = (hipStream_t)stream;
+    switch (d->dtype) {
+        case EQUIGSPR_F32: return eq::ff_backward<eq::kF32>(d, grad_y, zu, h, dzu, work, grads, st);
+        case EQUIGSPR_BF16: return eq::ff_backward<eq::kBF16>(d, grad_y, zu, h, dzu, work, grads, st);
+        default: return eq::ff_backward<eq::kF16>(d, grad_y, zu, h, dzu, work, grads, st);
+    }
+}

@@ -98,8 +98,13 @@ def unsorted_segment_mean(data, segment_ids, num_segments):
 
 # ------------------------------------------------------------------------------ pair model
 class CrossAttentionPoseRegression(nn.Module):
-    def __init__(self, egnn, num_nodes=2048, hidden_nf=33, device="cuda:0", variant="train", topk=None, fused_head=True):
+    def __init__(self, egnn, num_nodes=2048, hidden_nf=33, device="cuda:0", variant="train", topk=None, fused_head=True,
+                 context=None):
+        """``context`` (extension; the reference's model has none): a ``CloudContext`` applied to the EGNN's point features of both clouds
+        before the head.  Without it the model is the reference's, parameter for parameter."""
         super().__init__()
+        if context is not None and context.width != egnn.out_node_nf:
+            raise ValueError(f"context: width {context.width}, the EGNN gives {egnn.out_node_nf} features")
         self.fused_head = fused_head
         if variant not in ("train", "eval", "kitti"):
             raise ValueError("variant must be 'train', 'eval' or 'kitti'")
@@ -107,6 +112,7 @@ class CrossAttentionPoseRegression(nn.Module):
             topk = 2048 if variant == "kitti" else 128
         self.egnn, self.hidden_nf, self.num_nodes, self.device = egnn, hidden_nf, num_nodes, device
         self.variant, self.topk = variant, topk
+        self.context = context
         self.mlp = nn.Sequential(nn.Linear(2 * hidden_nf, hidden_nf), nn.ReLU(),
                                  nn.Linear(hidden_nf, hidden_nf // 2), nn.ReLU(),
                                  nn.Linear(hidden_nf // 2, 1))
@@ -140,6 +146,8 @@ class CrossAttentionPoseRegression(nn.Module):
             ea = torch.cat([ea_src.reshape(-1), ea_tgt.reshape(-1)], dim=0)
         h_o, x_o = self.egnn(h_all, x_all, graph, ea)
         Fo = h_o.shape[1]
+        if self.context is not None:
+            h_o = self.context(h_o.view(2, B, N, Fo)).view(2 * B * N, Fo)
         self._egnn_out = (h_o, x_o)
         return (h_o[:B * N].view(B, N, Fo), x_o[:B * N].view(B, N, 3), h_o[B * N:].view(B, N, Fo), x_o[B * N:].view(B, N, 3))
 
