@@ -23,19 +23,19 @@ struct AttnFwd {
 };
 
 template <int T, int W, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnFwd<T> a) {
+__global__ __launch_bounds__(NW * 64, W == 128 && T == kF32 ? 1 : 2) void attn_fwd_kernel(AttnFwd<T> a) {
     constexpr int KT = attn_tile<T, W>(), NT = NW * 64, ROWS = NW * 32, NP = Num<T>::planes;
     constexpr int KS = W / 16, DB = W / 32, KB = KT / 32;
-    constexpr float kShift = T == kF16 ? 10.f : 0.f;      // fp16: P is held as 2^10 P, so that probabilities down to 2^-34 count
+    // fp16: P is held as 2^8 P, so that probabilities down to 2^-32 count; with the slack that stays below 2^14
+    constexpr float kShift = T == kF16 ? 8.f : 0.f, kSlack = T == kF16 ? 6.f : 8.f;
     __shared__ __attribute__((aligned(16))) short tile_k[NP * KT * W];
     __shared__ __attribute__((aligned(16))) short tile_v[NP * KT * W];
     __shared__ __attribute__((aligned(16))) float hidden[KT];
     const AttnShape& s = a.s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    int id = xcd_block(blockIdx.x, gridDim.x);
-    const int rt = a.row_tiles - 1 - id % a.row_tiles;    // causal: the longest tiles first
-    id /= a.row_tiles;
-    const int split = id % a.splits, bh = id / a.splits, b = bh / s.kv_heads, hk = bh - b * s.kv_heads;
+    const AttnUnit un = attn_unit(s.batch * s.kv_heads, a.row_tiles * a.splits);
+    const int rt = a.row_tiles - 1 - un.unit / a.splits, split = un.unit % a.splits;      // causal: the longest tiles first
+    const int bh = un.bh, b = bh / s.kv_heads, hk = bh - b * s.kv_heads;
     const int ql = attn_len(s.q_lens, b, s.nq), kl = attn_len(s.kv_lens, b, s.nk);
     const int rows = s.nq * s.group, rows_valid = ql * s.group, row0 = rt * ROWS;
     const int row = row0 + wave * 32 + (lane & 31);
@@ -98,16 +98,24 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnFwd<T> a) {
                         if (h[i] != 0.f || k0 + j + i > limit) sc[kb][4 * g + i] = -INFINITY;
                 }
         }
-        float top = m;
+        float top = sc[0][0];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[kb][r]);
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float use = top == -INFINITY ? 0.f : top;   // nothing visible so far: P = exp2(-inf) = 0
-        const float old = exp2_fast((m - use) * s.scale_log2);
-        const float sub = kShift - use * s.scale_log2;
-        m = top;
+        // The reference value m only has to keep the exponentials in range: it follows the running maximum when that has risen by more
+        // than 2^kSlack, which is rare after the first tiles, and the accumulators are rescaled only then.
+        if (__any((top - m) * s.scale_log2 > kSlack)) {       // (-inf) - (-inf) is NaN: no
+            top = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+            const float old = top == -INFINITY ? 1.f : exp2_fast((m - top) * s.scale_log2);
+            m = top;
+            l *= old;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] *= old;
+        }
+        const float sub = m == -INFINITY ? 0.f : kShift - m * s.scale_log2;      // nothing visible so far: exp2(-inf) = 0
         float sum = 0.f;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -116,11 +124,7 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnFwd<T> a) {
                 sc[kb][r] = exp2_fast(fmaf(sc[kb][r], s.scale_log2, sub));
                 sum += sc[kb][r];
             }
-        l = fmaf(l, old, sum);
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[d][r] *= old;
+        l += sum;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll

@@ -22,7 +22,13 @@ struct AttnBwd {
     float* amax;                              // fp16: [2 * kAmaxBlocks]
     typename Num<T>::type *gq, *gk, *gv;      // contiguous, each may be null
     int row_tiles, key_tiles;
+    int key_splits, split_keys;               // attn_dq_kernel: parts of the key axis
+    int row_splits;                           // attn_dkv_kernel: parts of the row axis
+    float *part_q, *part_k, *part_v;          // [splits][the gradient's elements] when an axis is split
 };
+
+// rows of a staged tile: 64, or 32 where three planes or a wide head would take the registers of a second wave per SIMD
+template <int T, int W> constexpr int attn_bwd_tile() { return W == 128 || (T == kF32 && W == 64) ? 32 : 64; }
 
 // fp16: largest |dO| over the existing rows and |V| over the visible keys, one pair per workgroup
 template <int T>
@@ -71,22 +77,25 @@ __device__ __forceinline__ float attn_grad_scale(const AttnBwd<T>& a) {
     return ldexpf(1.f, e < -60 ? -60 : (e > 60 ? 60 : e));
 }
 
-template <int T, int W, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnBwd<T> a) {
-    constexpr int KT = attn_tile<T, W>(), NT = NW * 64, ROWS = NW * 32, NP = Num<T>::planes;
+constexpr int kBwdWaves = 4;                  // waves of a workgroup: each owns 32 rows (keys), all share the staged tiles
+
+template <int T, int W>
+__global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_kernel(AttnBwd<T> a) {
+    constexpr int KT = attn_bwd_tile<T, W>(), NT = kBwdWaves * 64, ROWS = kBwdWaves * 32, NP = Num<T>::planes;
     constexpr int KS = W / 16, DB = W / 32, KB = KT / 32;
     __shared__ __attribute__((aligned(16))) short tile_k[NP * KT * W];
     __shared__ __attribute__((aligned(16))) short tile_v[NP * KT * W];
     __shared__ __attribute__((aligned(16))) float hidden[KT];
     const AttnShape& s = a.s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const int id = xcd_block(blockIdx.x, gridDim.x);
-    const int rt = a.row_tiles - 1 - id % a.row_tiles, bh = id / a.row_tiles, b = bh / s.kv_heads, hk = bh - b * s.kv_heads;
+    const AttnUnit un = attn_unit(s.batch * s.kv_heads, a.row_tiles * a.key_splits);
+    const int rt = a.row_tiles - 1 - un.unit / a.key_splits, split = un.unit % a.key_splits, bh = un.bh, b = bh / s.kv_heads, hk = bh - b * s.kv_heads;
     const int ql = attn_len(s.q_lens, b, s.nq), kl = attn_len(s.kv_lens, b, s.nk);
     const int rows = s.nq * s.group, rows_valid = ql * s.group, row0 = rt * ROWS;
     const int row = row0 + wave * 32 + (lane & 31);
     const bool ok_row = row < rows_valid;
-    int k_end = kl;
+    const int k_begin = split * a.split_keys;
+    int k_end = min(kl, k_begin + a.split_keys);
     const int last_row = min(row0 + ROWS, rows_valid) - 1;
     if (s.causal && last_row >= 0) k_end = min(k_end, row_point(s, last_row) + kl - ql + 1);
     if (row0 >= rows_valid || !a.gq) k_end = 0;
@@ -111,7 +120,7 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnBwd<T> a) {
         }
     }
     delta += __shfl_xor(delta, 32);
-    if (row < rows && half == 0) a.delta[at] = delta;
+    if (row < rows && half == 0 && split == 0) a.delta[at] = delta;
     if (!a.gq) return;
     const float lse = ok_row ? a.lse[at] : INFINITY;
     const float factor = attn_grad_scale<T>(a);
@@ -129,8 +138,8 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnBwd<T> a) {
         sv.load([&](int j) { return ok(j) ? key_row(a.v, b, hk, k0 + j) : nullptr; }, s.dim);
         if (threadIdx.x < KT) vis = ok(threadIdx.x);
     };
-    if (k_end > 0) load_tile(0);
-    for (int k0 = 0; k0 < k_end; k0 += KT) {
+    if (k_begin < k_end) load_tile(k_begin);
+    for (int k0 = k_begin; k0 < k_end; k0 += KT) {
         __syncthreads();
         sk.store(tile_k);
         sv.store(tile_v);
@@ -173,7 +182,8 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnBwd<T> a) {
     if (row >= rows) return;
     const float back = s.scale / factor;
     const int i0 = row_point(s, row);
-    typename Num<T>::type* o = a.gq + (((int64_t)b * s.nq + i0) * s.heads + hk * s.group + row - i0 * s.group) * s.dim;
+    const int64_t o = (((int64_t)b * s.nq + i0) * s.heads + hk * s.group + row - i0 * s.group) * s.dim;
+    float* part = a.key_splits > 1 ? a.part_q + split * (int64_t)s.batch * s.nq * s.heads * s.dim : nullptr;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -182,13 +192,14 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnBwd<T> a) {
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = acc[d][4 * gq + i] * back;
-            store4<T>(o + c, x, s.dim - c);
+            if (part) store4<kF32>(part + o + c, x, s.dim - c);
+            else store4<T>(a.gq + o + c, x, s.dim - c);
         }
 }
 
-template <int T, int W, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnBwd<T> a) {
-    constexpr int RT = attn_tile<T, W>(), NT = NW * 64, KEYS = NW * 32, NP = Num<T>::planes;
+template <int T, int W>
+__global__ __launch_bounds__(kBwdWaves * 64, T == kF32 || W == 128 ? 1 : 2) void attn_dkv_kernel(AttnBwd<T> a) {
+    constexpr int RT = attn_bwd_tile<T, W>(), NT = kBwdWaves * 64, KEYS = kBwdWaves * 32, NP = Num<T>::planes;
     constexpr int KS = W / 16, DB = W / 32, RB = RT / 32;
     constexpr float kShift = T == kF16 ? 10.f : 0.f;
     __shared__ __attribute__((aligned(16))) short tile_q[NP * RT * W];
@@ -198,14 +209,16 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnBwd<T> a) {
     __shared__ __attribute__((aligned(16))) int row_limit[RT];
     const AttnShape& s = a.s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const int id = xcd_block(blockIdx.x, gridDim.x);
-    const int kt = id % a.key_tiles, bh = id / a.key_tiles, b = bh / s.kv_heads, hk = bh - b * s.kv_heads;
+    const AttnUnit un = attn_unit(s.batch * s.kv_heads, a.key_tiles * a.row_splits);
+    const int kt = un.unit / a.row_splits, split = un.unit % a.row_splits, bh = un.bh, b = bh / s.kv_heads, hk = bh - b * s.kv_heads;
     const int ql = attn_len(s.q_lens, b, s.nq), kl = attn_len(s.kv_lens, b, s.nk);
     const int rows = s.nq * s.group, rows_valid = ql * s.group, key0 = kt * KEYS;
     const int key = key0 + wave * 32 + (lane & 31);
     const bool ok_key = key < kl && (!s.key_mask || s.key_mask[b * s.mask_stride + key]);
-    const int r_end = key0 < kl ? rows_valid : 0;
-    const int r_begin = s.causal ? max(0, key0 - kl + ql) * s.group : 0;      // the first point that sees this tile's first key
+    // the rows from the first point that sees this tile's first key, cut into equal parts
+    const int r_first = s.causal ? max(0, key0 - kl + ql) * s.group : 0, r_count = key0 < kl ? max(0, rows_valid - r_first) : 0;
+    const int r_part = ((r_count + a.row_splits - 1) / a.row_splits + RT - 1) / RT * RT;
+    const int r_begin = r_first + split * r_part, r_end = min(r_first + r_count, r_begin + r_part);
 
     Op8<T> k[KS], v[KS];                      // keys that are not visible: zeros; their lanes' results are replaced at the end
     {
@@ -291,6 +304,7 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnBwd<T> a) {
     if (key >= s.nk) return;
     const float back_k = s.scale / factor, back_v = exp2_fast(-kShift);
     const int64_t o = (((int64_t)b * s.nk + key) * s.kv_heads + hk) * s.dim;
+    const int64_t part = a.row_splits > 1 ? split * (int64_t)s.batch * s.nk * s.kv_heads * s.dim : -1;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -302,36 +316,85 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnBwd<T> a) {
                 x[i] = ok_key ? acc_k[d][4 * gr + i] * back_k : 0.f;
                 y[i] = ok_key ? acc_v[d][4 * gr + i] * back_v : 0.f;
             }
-            if (a.gk) store4<T>(a.gk + o + c, x, s.dim - c);
-            if (a.gv) store4<T>(a.gv + o + c, y, s.dim - c);
+            if (part >= 0) {
+                if (a.gk) store4<kF32>(a.part_k + part + o + c, x, s.dim - c);
+                if (a.gv) store4<kF32>(a.part_v + part + o + c, y, s.dim - c);
+            } else {
+                if (a.gk) store4<T>(a.gk + o + c, x, s.dim - c);
+                if (a.gv) store4<T>(a.gv + o + c, y, s.dim - c);
+            }
         }
 }
 
-// Four waves share a tile when that still gives every compute unit a workgroup; one wave otherwise (shorter runs, more of them).
-static int attn_bwd_waves(int64_t owned, int64_t heads) { return ceil_div(owned, 128) * heads >= 256 ? 4 : 1; }
+// a gradient as the sum of its parts, in order; the two gradients of keys and values in one launch
+template <int T>
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float* part0, const float* part1, int splits, int64_t n, typename Num<T>::type* out0,
+                                                       typename Num<T>::type* out1) {
+    const float* part = blockIdx.y ? part1 : part0;
+    typename Num<T>::type* out = blockIdx.y ? out1 : out0;
+    if (!out) return;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < splits; ++p)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i + e < n) v[e] += part[p * n + i + e];
+        store4<T>(out + i, v, (int)(n - i < 4 ? n - i : 4));
+    }
+}
+
+// Parts: the owned axis alone gives too few workgroups when it is short, and a causal mask leaves the first keys with all the work, so the
+// other axis is cut until there are two workgroups per compute unit (causal: four), into parts of at least 256.
+static int attn_bwd_splits(int64_t tiles, int64_t length, int64_t want) {
+    if (tiles == 0 || tiles >= want) return 1;
+    const int64_t most = (length + 255) / 256, s = want / tiles;
+    return (int)(s < most ? (s > 1 ? s : 1) : (most > 1 ? most : 1));
+}
+
+struct AttnBwdPlan { int row_tiles, key_tiles, key_splits, split_keys, row_splits; int64_t delta, parts_q, parts_k; };
+static AttnBwdPlan attn_bwd_plan(const AttnShape& s) {
+    constexpr int kOwned = kBwdWaves * 32;
+    AttnBwdPlan p;
+    const int64_t heads = (int64_t)s.batch * s.kv_heads, rows = (int64_t)s.nq * s.group;
+    p.row_tiles = ceil_div(rows, kOwned);
+    p.key_tiles = ceil_div(s.nk, kOwned);
+    p.key_splits = attn_bwd_splits(p.row_tiles * heads, s.nk, 512);
+    p.split_keys = ceil_div(ceil_div(s.nk, p.key_splits), 64) * 64;
+    p.key_splits = s.nk ? ceil_div(s.nk, p.split_keys) : 1;
+    p.row_splits = attn_bwd_splits(p.key_tiles * heads, rows, s.causal ? 1024 : 512);
+    p.delta = (heads * rows + 3) / 4 * 4;
+    p.parts_q = p.key_splits > 1 ? p.key_splits * heads * rows * s.dim : 0;
+    p.parts_k = p.row_splits > 1 ? p.row_splits * heads * s.nk * s.dim : 0;
+    return p;
+}
 
 template <int T, int W>
-static int attn_bwd_launch(AttnBwd<T>& a, hipStream_t st) {
+static int attn_bwd_launch(const AttnBwd<T>& a, hipStream_t st) {
     const AttnShape& s = a.s;
     const int64_t heads = (int64_t)s.batch * s.kv_heads;
-    const int wq = attn_bwd_waves((int64_t)s.nq * s.group, heads), wk = attn_bwd_waves(s.nk, heads);
-    a.row_tiles = ceil_div((int64_t)s.nq * s.group, 32 * wq);
-    a.key_tiles = ceil_div(s.nk, 32 * wk);
-    const int64_t bq = a.row_tiles * heads, bk = a.key_tiles * heads;
+    const int64_t bq = (int64_t)a.row_tiles * a.key_splits * heads, bk = (int64_t)a.key_tiles * a.row_splits * heads;
     EQ_CHECK_ARG(bq < (1 << 24) && bk < (1 << 24), EQUIGSPR_ENOTSUP, "attention_backward: more workgroups than one launch takes");
     if (T == kF16) {
         attn_amax_kernel<T><<<kAmaxBlocks, 256, 0, st>>>(a);
         EQ_CHECK_LAUNCH("attention_backward (range)");
     }
     if (bq) {
-        if (wq == 1) attn_dq_kernel<T, W, 1><<<(unsigned)bq, 64, 0, st>>>(a);
-        else attn_dq_kernel<T, W, 4><<<(unsigned)bq, 256, 0, st>>>(a);
+        attn_dq_kernel<T, W><<<(unsigned)bq, kBwdWaves * 64, 0, st>>>(a);
         EQ_CHECK_LAUNCH("attention_backward (rows)");
+        if (a.key_splits > 1 && a.gq) {
+            const int64_t n = heads * s.nq * s.group * s.dim, blocks = ceil_div(n, 1024);
+            attn_sum_kernel<T><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(a.part_q, nullptr, a.key_splits, n, a.gq, nullptr);
+            EQ_CHECK_LAUNCH("attention_backward (rows' parts)");
+        }
     }
     if (bk && (a.gk || a.gv)) {
-        if (wk == 1) attn_dkv_kernel<T, W, 1><<<(unsigned)bk, 64, 0, st>>>(a);
-        else attn_dkv_kernel<T, W, 4><<<(unsigned)bk, 256, 0, st>>>(a);
+        attn_dkv_kernel<T, W><<<(unsigned)bk, kBwdWaves * 64, 0, st>>>(a);
         EQ_CHECK_LAUNCH("attention_backward (keys)");
+        if (a.row_splits > 1) {
+            const int64_t n = heads * s.nk * s.dim, blocks = ceil_div(n, 1024);
+            attn_sum_kernel<T><<<dim3((unsigned)(blocks < 4096 ? blocks : 4096), 2), 256, 0, st>>>(a.part_k, a.part_v, a.row_splits, n, a.gk, a.gv);
+            EQ_CHECK_LAUNCH("attention_backward (keys' parts)");
+        }
     }
     return 0;
 }
@@ -350,7 +413,11 @@ static int attn_bwd(const equigspr_attention* d, const AttnShape& s, const void*
     a.o = attn_tensor<T>(o, s.dim);
     a.lse = lse;
     a.amax = work;
+    const AttnBwdPlan p = attn_bwd_plan(s);
     a.delta = work + 2 * kAmaxBlocks;
+    a.part_q = a.part_k = a.delta + p.delta;  // the rows' parts are summed before the keys' parts are written
+    a.part_v = a.part_k + p.parts_k;
+    a.row_tiles = p.row_tiles; a.key_tiles = p.key_tiles; a.key_splits = p.key_splits; a.split_keys = p.split_keys; a.row_splits = p.row_splits;
     a.gq = (E*)gq; a.gk = (E*)gk; a.gv = (E*)gv;
     return s.dim <= 32 ? attn_bwd_launch<T, 32>(a, st) : s.dim <= 64 ? attn_bwd_launch<T, 64>(a, st) : attn_bwd_launch<T, 128>(a, st);
 }
@@ -360,7 +427,8 @@ static int attn_bwd(const equigspr_attention* d, const AttnShape& s, const void*
 extern "C" int64_t equigspr_attention_backward_work_size(const equigspr_attention* d) {
     eq::AttnShape s;
     if (eq::attn_shape(d, &s) != 0) return -1;
-    return 2 * eq::kAmaxBlocks + (int64_t)s.batch * s.kv_heads * s.nq * s.group;
+    const eq::AttnBwdPlan p = eq::attn_bwd_plan(s);
+    return 2 * eq::kAmaxBlocks + p.delta + (p.parts_q > 2 * p.parts_k ? p.parts_q : 2 * p.parts_k);
 }
 
 extern "C" int equigspr_attention_backward(const equigspr_attention* d, const void* out, const float* lse, const equigspr_attention_tensor* grad_out,
