@@ -28,8 +28,8 @@ __global__ __launch_bounds__(NW * 64, W == 128 && T == kF32 ? 1 : 2) void attn_f
     constexpr int KS = W / 16, DB = W / 32, KB = KT / 32;
     // fp16: P is held as 2^8 P, so that probabilities down to 2^-32 count; with the slack that stays below 2^14
     constexpr float kShift = T == kF16 ? 8.f : 0.f, kSlack = T == kF16 ? 6.f : 8.f;
-    __shared__ __attribute__((aligned(16))) short tile_k[NP * KT * W];
-    __shared__ __attribute__((aligned(16))) short tile_v[NP * KT * W];
+    __shared__ __attribute__((aligned(16))) short tile_k[NP * Tile<W>::size(KT)];
+    __shared__ __attribute__((aligned(16))) short tile_v[NP * Tile<W>::size(KT)];
     __shared__ __attribute__((aligned(16))) float hidden[KT];
     const AttnShape& s = a.s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;

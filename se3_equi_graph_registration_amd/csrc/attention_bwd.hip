@@ -83,8 +83,8 @@ template <int T, int W>
 __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_kernel(AttnBwd<T> a) {
     constexpr int KT = attn_bwd_tile<T, W>(), NT = kBwdWaves * 64, ROWS = kBwdWaves * 32, NP = Num<T>::planes;
     constexpr int KS = W / 16, DB = W / 32, KB = KT / 32;
-    __shared__ __attribute__((aligned(16))) short tile_k[NP * KT * W];
-    __shared__ __attribute__((aligned(16))) short tile_v[NP * KT * W];
+    __shared__ __attribute__((aligned(16))) short tile_k[NP * Tile<W>::size(KT)];
+    __shared__ __attribute__((aligned(16))) short tile_v[NP * Tile<W>::size(KT)];
     __shared__ __attribute__((aligned(16))) float hidden[KT];
     const AttnShape& s = a.s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -198,15 +198,18 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_ker
 }
 
 template <int T, int W>
-__global__ __launch_bounds__(kBwdWaves * 64, T == kF32 || W == 128 ? 1 : 2) void attn_dkv_kernel(AttnBwd<T> a) {
+__global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dkv_kernel(AttnBwd<T> a) {
     constexpr int RT = attn_bwd_tile<T, W>(), NT = kBwdWaves * 64, KEYS = kBwdWaves * 32, NP = Num<T>::planes;
     constexpr int KS = W / 16, DB = W / 32, RB = RT / 32;
     constexpr float kShift = T == kF16 ? 10.f : 0.f;
-    __shared__ __attribute__((aligned(16))) short tile_q[NP * RT * W];
-    __shared__ __attribute__((aligned(16))) short tile_g[NP * RT * W];
+    __shared__ __attribute__((aligned(16))) short tile_q[NP * Tile<W>::size(RT)];
+    __shared__ __attribute__((aligned(16))) short tile_g[NP * Tile<W>::size(RT)];
     __shared__ __attribute__((aligned(16))) float row_lse[RT];
     __shared__ __attribute__((aligned(16))) float row_delta[RT];
     __shared__ __attribute__((aligned(16))) int row_limit[RT];
+    // wide 16-bit heads: V waits in LDS, its registers make room for a second wave per SIMD
+    constexpr bool kKeepV = !(W == 128 && NP == 1);
+    __shared__ __attribute__((aligned(16))) short own_v[kKeepV ? 8 : Tile<W>::size(KEYS)];
     const AttnShape& s = a.s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const AttnUnit un = attn_unit(s.batch * s.kv_heads, a.key_tiles * a.row_splits);
@@ -220,7 +223,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 || W == 128 ? 1 : 2) void
     const int r_part = ((r_count + a.row_splits - 1) / a.row_splits + RT - 1) / RT * RT;
     const int r_begin = r_first + split * r_part, r_end = min(r_first + r_count, r_begin + r_part);
 
-    Op8<T> k[KS], v[KS];                      // keys that are not visible: zeros; their lanes' results are replaced at the end
+    Op8<T> k[KS], v[kKeepV ? KS : 1];                      // keys that are not visible: zeros; their lanes' results are replaced at the end
     {
         const typename Num<T>::type* pk = ok_key ? key_row(a.k, b, hk, key) : nullptr;
         const typename Num<T>::type* pv = ok_key ? key_row(a.v, b, hk, key) : nullptr;
@@ -228,7 +231,9 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 || W == 128 ? 1 : 2) void
         for (int ks = 0; ks < KS; ++ks) {
             const int c = ks * 16 + half * 8;
             k[ks] = planes_of<T>(ok_key ? load8<T>(pk, c, s.dim) : raw_zero<T>());
-            v[ks] = planes_of<T>(ok_key ? load8<T>(pv, c, s.dim) : raw_zero<T>());
+            const Op8<T> o = planes_of<T>(ok_key ? load8<T>(pv, c, s.dim) : raw_zero<T>());
+            if constexpr (kKeepV) v[ks] = o;
+            else *reinterpret_cast<s16x8*>(own_v + Tile<W>::at(wave * 32 + (lane & 31), 2 * ks + half)) = o.p[0];
         }
     }
     const float factor = attn_grad_scale<T>(a), fs = factor * exp2_fast(-kShift);
@@ -269,7 +274,10 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 || W == 128 ? 1 : 2) void
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 mma<T>(sc, tile_rows<T, W, RT>(tile_q, rb * 32, ks, lane), k[ks]);
-                mma<T>(dp, tile_rows<T, W, RT>(tile_g, rb * 32, ks, lane), v[ks]);
+                Op8<T> ov;
+                if constexpr (kKeepV) ov = v[ks];
+                else ov.p[0] = Tile<W>::row8(own_v, wave * 32 + (lane & 31), 2 * ks + half);      // written by this wave
+                mma<T>(dp, tile_rows<T, W, RT>(tile_g, rb * 32, ks, lane), ov);
             }
 #pragma unroll
             for (int gr = 0; gr < 4; ++gr) {

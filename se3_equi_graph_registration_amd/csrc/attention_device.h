@@ -49,7 +49,7 @@ __device__ __forceinline__ typename Num<T>::type* key_row(const AttnTensor<T>& t
 // loads are in flight under this tile's products
 template <int T, int W, int ROWS, int NT>
 struct Stager {
-    static constexpr int kChunks = W / 8, kPer = ROWS * kChunks / NT, kPlane = ROWS * W;      // chunks of a row, of a thread; values of a plane
+    static constexpr int kChunks = W / 8, kPer = ROWS * kChunks / NT, kPlane = Tile<W>::size(ROWS);      // chunks of a row, of a thread; values of a plane
     static_assert(kPer * NT == ROWS * kChunks, "whole chunks per thread");
     Raw8<T> raw[kPer];
     // row_of(r) -> pointer of row r, or null for a row of zeros
@@ -79,7 +79,7 @@ template <int T, int W, int ROWS>
 __device__ __forceinline__ Op8<T> tile_rows(const short* tile, int row0, int ks, int lane) {
     Op8<T> o;
 #pragma unroll
-    for (int p = 0; p < Num<T>::planes; ++p) o.p[p] = Tile<W>::row8(tile + p * ROWS * W, row0 + (lane & 31), 2 * ks + (lane >> 5));
+    for (int p = 0; p < Num<T>::planes; ++p) o.p[p] = Tile<W>::row8(tile + p * Tile<W>::size(ROWS), row0 + (lane & 31), 2 * ks + (lane >> 5));
     return o;
 }
 // A operand of the transposed tile: 32 columns from col0 as rows; the contraction runs over the 16 tile rows from row0 in the order in
@@ -91,7 +91,7 @@ __device__ __forceinline__ Op8<T> tile_cols(const short* tile, int row0, int col
     const int r = row0 + 4 * (lane >> 5), c = col0 + (lane & 16);
 #pragma unroll
     for (int p = 0; p < Num<T>::planes; ++p)
-        o.p[p] = join8(Tile<W>::col4(tile + p * ROWS * W, r, c, lane), Tile<W>::col4(tile + p * ROWS * W, r + 8, c, lane));
+        o.p[p] = join8(Tile<W>::col4(tile + p * Tile<W>::size(ROWS), r, c, lane), Tile<W>::col4(tile + p * Tile<W>::size(ROWS), r + 8, c, lane));
     return o;
 }
 

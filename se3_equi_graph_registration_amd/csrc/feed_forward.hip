@@ -64,7 +64,7 @@ template <int T> constexpr int ff_k_tile() { return T == kF32 ? 32 : 64; }
 template <int T, bool kAcross>
 struct FfTile {
     static constexpr int BK = ff_k_tile<T>(), W = kAcross ? kFfTile : BK, ROWS = kAcross ? BK : kFfTile;
-    static constexpr int kPlane = W * ROWS, kPer = ROWS * W / 8 / 256;
+    static constexpr int kPlane = Tile<W>::size(ROWS), kPer = ROWS * W / 8 / 256;
     Raw8<T> raw[kPer];
     // outer0: first output row / column of the tile; k0: first contraction index; k_end bounds it
     template <class F>

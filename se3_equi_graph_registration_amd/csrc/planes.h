@@ -152,20 +152,17 @@ __device__ __forceinline__ Raw8<T> load8(const typename Num<T>::type* row, int c
     return r;
 }
 
-// A tile of rows of W 16-bit values in LDS.  Rows are unpadded; the 16-byte chunk c of row r lies at c ^ swz(r), chosen so that both
-// reads below touch every bank once: the 16 rows of a ds_read_b128 group differ in their (bank half, chunk), and the four rows of a
-// transposed read lie in four different quarters.  W = 32, 64 or 128 (rows of 16, 32, 64 banks).
+// A tile of rows of W 16-bit values in LDS.  The rows' stride is padded so that the 16 rows of a ds_read_b128 group start in 16 different
+// bank quads; the four rows of a transposed read then overlap two-fold, which costs a cycle.  (An XOR swizzle has neither conflict but an
+// address register per k-step: in the kernels' keys' gradients at W = 128 that was the difference between one and two waves per SIMD.)
 template <int W>
 struct Tile {
     static_assert(W == 32 || W == 64 || W == 128, "tile width");
-    static constexpr int kChunks = W / 8;
-    __device__ static __forceinline__ int swz(int r) {
-        if constexpr (W == 32) return (r >> 2) & 3;
-        else if constexpr (W == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
-        else return ((r & 3) << 2) | ((r >> 2) & 3);
-    }
+    static constexpr int kStride = W == 32 ? 40 : W == 64 ? 72 : 152;
+    // values of a tile of `rows` rows
+    __host__ __device__ static constexpr int size(int rows) { return rows * kStride; }
     // offset (in 16-bit values) of chunk c of row r
-    __device__ static __forceinline__ int at(int r, int c) { return (r * kChunks + (c ^ swz(r))) * 8; }
+    __device__ static __forceinline__ int at(int r, int c) { return r * kStride + c * 8; }
     // eight consecutive values of one row
     __device__ static __forceinline__ s16x8 row8(const short* t, int r, int c) { return *reinterpret_cast<const s16x8*>(t + at(r, c)); }
     // transposed: lane l receives the values of rows r0 .. r0 + 3 in column col0 + (l & 15); r0 % 4 == 0, col0 % 16 == 0 (both may
