@@ -16,13 +16,18 @@ from . import _lib
 from .ops import DTYPE_CODES, _p, _stream, check_capture, need_float, on_device, wants_grad
 
 
+def _stride(t, axis):
+    return t.stride(axis) if t.shape[axis] > 1 else 0
+
+
 def _rows(t):
-    """The kernels walk rows of unit stride; any other stride is taken as it is."""
-    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+    """The kernels walk rows of unit stride, points and heads less than 2^31 / 128 bytes apart; any other stride is taken as it is."""
+    near = (_stride(t, 1) + _stride(t, 2)) * 128 * t.element_size() < 1 << 31
+    return t if near and (t.shape[-1] == 1 or t.stride(-1) == 1) else t.contiguous()
 
 
 def _tensor(t):
-    return _lib.AttentionTensor(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+    return _lib.AttentionTensor(t.data_ptr(), _stride(t, 0), _stride(t, 1), _stride(t, 2))
 
 
 def _describe(q, k, v, q_lens, kv_lens, key_mask, causal, scale):

@@ -62,8 +62,17 @@ __global__ __launch_bounds__(NW * 64, W == 128 && T == kF32 ? 1 : 2) void attn_f
     float m = -INFINITY, l = 0.f;
 
     Stager<T, W, KT, NT> sk, sv;
+    sk.init([&](int j) { return j * (int)a.k.sn; });
+    sv.init([&](int j) { return j * (int)a.v.sn; });
     bool vis = false;
+    const bool even = !mask && s.dim % 8 == 0;
     auto load_tile = [&](int k0) {
+        if (even && k0 + KT <= k_end) {
+            sk.load_whole(key_row(a.k, b, hk, k0), s.dim);
+            sv.load_whole(key_row(a.v, b, hk, k0), s.dim);
+            vis = true;
+            return;
+        }
         auto ok = [&](int j) { return k0 + j < k_end && (!mask || mask[k0 + j]); };
         sk.load([&](int j) { return ok(j) ? key_row(a.k, b, hk, k0 + j) : nullptr; }, s.dim);
         sv.load([&](int j) { return ok(j) ? key_row(a.v, b, hk, k0 + j) : nullptr; }, s.dim);
@@ -257,6 +266,9 @@ int attn_shape(const equigspr_attention* d, AttnShape* s) {
     const int64_t g = d->heads / d->kv_heads;
     EQ_CHECK_ARG(d->nq * g * g < (1ll << 32) && d->nq * g < (1ll << 30) && d->nk < (1 << 30) && (int64_t)d->batch * d->heads < (1 << 24), EQUIGSPR_ENOTSUP,
                  "attention: too many rows, keys or heads for one call");
+    const int esize = d->dtype == EQUIGSPR_F32 ? 4 : 2;
+    EQ_CHECK_ARG(attn_near(d->q, esize) && attn_near(d->k, esize) && attn_near(d->v, esize), EQUIGSPR_ENOTSUP,
+                 "attention: negative strides, or points or heads further apart than 2^31 / 128 bytes");
     EQ_CHECK_ARG(!d->batch || ((d->q.data || !d->nq) && ((d->k.data && d->v.data) || !d->nk)), EQUIGSPR_EINVAL, "attention: null tensor");
     s->batch = d->batch; s->nq = d->nq; s->nk = d->nk; s->heads = d->heads; s->kv_heads = d->kv_heads; s->group = (int)g; s->dim = d->dim;
     s->group_magic = (unsigned)(((1ull << 32) + g - 1) / g);

@@ -131,8 +131,17 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_ker
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
 
     Stager<T, W, KT, NT> sk, sv;
+    sk.init([&](int j) { return j * (int)a.k.sn; });
+    sv.init([&](int j) { return j * (int)a.v.sn; });
     bool vis = false;
+    const bool even = !mask && s.dim % 8 == 0;
     auto load_tile = [&](int k0) {
+        if (even && k0 + KT <= k_end) {
+            sk.load_whole(key_row(a.k, b, hk, k0), s.dim);
+            sv.load_whole(key_row(a.v, b, hk, k0), s.dim);
+            vis = true;
+            return;
+        }
         auto ok = [&](int j) { return k0 + j < k_end && (!mask || mask[k0 + j]); };
         sk.load([&](int j) { return ok(j) ? key_row(a.k, b, hk, k0 + j) : nullptr; }, s.dim);
         sv.load([&](int j) { return ok(j) ? key_row(a.v, b, hk, k0 + j) : nullptr; }, s.dim);
@@ -158,6 +167,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_ker
                 mma<T>(dp, tile_rows<T, W, KT>(tile_v, kb * 32, ks, lane), g[ks]);
             }
             if (edge) {
+                asm volatile("");                         // a branch: as selects this would be a third of the tile's arithmetic
 #pragma unroll
                 for (int gq = 0; gq < 4; ++gq) {
                     const int j = kb * 32 + 8 * gq + 4 * half;
@@ -244,11 +254,19 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dkv_ke
         for (int r = 0; r < 16; ++r) acc_k[d][r] = acc_v[d][r] = 0.f;
 
     Stager<T, W, RT, NT> sq, sg;
+    sq.init([&](int r) { const int i = row_point(s, r); return i * (int)a.q.sn + (r - i * s.group) * (int)a.q.sh; });
+    sg.init([&](int r) { const int i = row_point(s, r); return i * (int)a.g.sn + (r - i * s.group) * (int)a.g.sh; });
+    const bool even = RT % s.group == 0 && s.dim % 8 == 0;       // tiles then begin with the first head of a group
     float my_lse = INFINITY, my_delta = 0.f;
     int my_limit = -1;
     auto load_tile = [&](int r0) {
-        sq.load([&](int r) { return r0 + r < r_end ? packed_row(a.q, s, b, hk, r0 + r) : nullptr; }, s.dim);
-        sg.load([&](int r) { return r0 + r < r_end ? packed_row(a.g, s, b, hk, r0 + r) : nullptr; }, s.dim);
+        if (even && r0 + RT <= r_end) {
+            sq.load_whole(packed_row(a.q, s, b, hk, r0), s.dim);
+            sg.load_whole(packed_row(a.g, s, b, hk, r0), s.dim);
+        } else {
+            sq.load([&](int r) { return r0 + r < r_end ? packed_row(a.q, s, b, hk, r0 + r) : nullptr; }, s.dim);
+            sg.load([&](int r) { return r0 + r < r_end ? packed_row(a.g, s, b, hk, r0 + r) : nullptr; }, s.dim);
+        }
         if (threadIdx.x < RT) {
             const int r = r0 + threadIdx.x;
             const int64_t at = (int64_t)bh * rows + r;
@@ -289,11 +307,14 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dkv_ke
                     sc[4 * gr + i] = p;
                     dp[4 * gr + i] = p * (dp[4 * gr + i] - del[i]) * fs;
                 }
-                if (edge) {
+            }
+            if (edge) {
+                asm volatile("");                         // a branch, see above
+#pragma unroll
+                for (int gr = 0; gr < 4; ++gr)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (key > row_limit[r + i]) sc[4 * gr + i] = dp[4 * gr + i] = 0.f;
-                }
+                        if (key > row_limit[rb * 32 + 8 * gr + 4 * half + i]) sc[4 * gr + i] = dp[4 * gr + i] = 0.f;
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -444,6 +465,7 @@ extern "C" int equigspr_attention_backward(const equigspr_attention* d, const vo
     eq::AttnShape s;
     if (const int rc = eq::attn_shape(d, &s)) return rc;
     EQ_CHECK_ARG(grad_out && work, EQUIGSPR_EINVAL, "attention_backward: grad_out or work is null");
+    EQ_CHECK_ARG(eq::attn_near(*grad_out, d->dtype == EQUIGSPR_F32 ? 4 : 2), EQUIGSPR_ENOTSUP, "attention_backward: strides of grad_out out of range");
     EQ_CHECK_ARG(!s.batch || !s.nq || (out && lse && grad_out->data), EQUIGSPR_EINVAL, "attention_backward: out, lse or grad_out is null");
     if (s.batch == 0) return 0;
     hipStream_t st = (hipStream_t)stream;

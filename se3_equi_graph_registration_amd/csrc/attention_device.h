@@ -46,19 +46,39 @@ __device__ __forceinline__ typename Num<T>::type* key_row(const AttnTensor<T>& t
 }
 
 // ROWS x W values from memory to the planes of a tile by NT threads: load() to registers, store() to LDS, so that the next tile's
-// loads are in flight under this tile's products
+// loads are in flight under this tile's products.  A thread's chunks all lie in one column of chunks.
 template <int T, int W, int ROWS, int NT>
 struct Stager {
+    using E = typename Num<T>::type;
     static constexpr int kChunks = W / 8, kPer = ROWS * kChunks / NT, kPlane = Tile<W>::size(ROWS);      // chunks of a row, of a thread; values of a plane
-    static_assert(kPer * NT == ROWS * kChunks, "whole chunks per thread");
+    static_assert(kPer * NT == ROWS * kChunks && NT % kChunks == 0, "whole chunks per thread");
     Raw8<T> raw[kPer];
+    unsigned off[kPer];                       // of the thread's chunks from the tile's first row, when rows lie at fixed distances
+    // row_off(r): distance of row r of a tile from its first row, in values, below 2^31 bytes (host check)
+    template <class F>
+    __device__ __forceinline__ void init(F row_off) {
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+            const int id = threadIdx.x + u * NT;
+            off[u] = (unsigned)((row_off(id / kChunks) + (id % kChunks) * 8) * (int)sizeof(E));
+        }
+    }
+    // a whole tile of existing rows, width % 8 == 0: one base in scalar registers, the threads' offsets computed once
+    __device__ __forceinline__ void load_whole(const E* first_row, int width) {
+        const bool in = (int)(threadIdx.x % kChunks) * 8 < width;
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+            if (!in) raw[u] = raw_zero<T>();
+            else raw[u] = load8<T>(reinterpret_cast<const E*>(reinterpret_cast<const char*>(first_row) + off[u]), 0, 8);
+        }
+    }
     // row_of(r) -> pointer of row r, or null for a row of zeros
     template <class F>
     __device__ __forceinline__ void load(F row_of, int width) {
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
             const int id = threadIdx.x + u * NT;
-            const typename Num<T>::type* row = row_of(id / kChunks);
+            const E* row = row_of(id / kChunks);
             raw[u] = row ? load8<T>(row, (id % kChunks) * 8, width) : raw_zero<T>();
         }
     }
@@ -121,6 +141,11 @@ static inline AttnTensor<T> attn_tensor(const equigspr_attention_tensor& t, int 
     r.p = (E*)t.data;
     r.sb = t.stride_batch; r.sn = t.stride_point; r.sh = t.stride_head;
     return r;
+}
+
+// rows of a tile lie within 2^31 bytes of each other (the kernels' 32-bit offsets inside a tile)
+static inline bool attn_near(const equigspr_attention_tensor& t, int esize) {
+    return (t.stride_point * 128 + t.stride_head * 128) * esize < (1ll << 31) && t.stride_batch >= 0 && t.stride_point >= 0 && t.stride_head >= 0;
 }
 
 // checks the description and derives what the kernels use; 0 or an error code
