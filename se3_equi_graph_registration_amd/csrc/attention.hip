@@ -22,10 +22,11 @@ struct AttnFwd {
     float* part_l;                            // [splits][batch * kv_heads][nq * group], -inf for a part without keys
 };
 
-template <int T, int W, int NW>
+// W: width of the staged tiles, KS: steps of 16 that the head dim takes in them
+template <int T, int W, int KS, int NW>
 __global__ __launch_bounds__(NW * 64, W == 128 && T == kF32 ? 1 : 2) void attn_fwd_kernel(AttnFwd<T> a) {
     constexpr int KT = attn_tile<T, W>(), NT = NW * 64, ROWS = NW * 32, NP = Num<T>::planes;
-    constexpr int KS = W / 16, DB = W / 32, KB = KT / 32;
+    constexpr int DB = (KS + 1) / 2, KB = KT / 32;
     // fp16: P is held as 2^8 P, so that probabilities down to 2^-32 count; with the slack that stays below 2^14
     constexpr float kShift = T == kF16 ? 8.f : 0.f, kSlack = T == kF16 ? 6.f : 8.f;
     __shared__ __attribute__((aligned(16))) short tile_k[NP * Tile<W>::size(KT)];
@@ -87,6 +88,7 @@ __global__ __launch_bounds__(NW * 64, W == 128 && T == kF32 ? 1 : 2) void attn_f
         __syncthreads();
         if (k0 + KT < k_end) load_tile(k0 + KT);
         pf32x16 sc[KB];
+        __builtin_amdgcn_s_setprio(1);                    // a wave with products to issue goes before one in its softmax
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -94,6 +96,7 @@ __global__ __launch_bounds__(NW * 64, W == 128 && T == kF32 ? 1 : 2) void attn_f
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) mma<T>(sc[kb], tile_rows<T, W, KT>(tile_k, kb * 32, ks, lane), q[ks]);
         }
+        __builtin_amdgcn_s_setprio(0);
         const bool edge = mask || k0 + KT > k_end || (s.causal && k0 + KT > row_point(s, row0 + wave * 32) + kl - ql + 1);
         if (edge) {
 #pragma unroll
@@ -182,28 +185,33 @@ __global__ __launch_bounds__(NW * 64, W == 128 && T == kF32 ? 1 : 2) void attn_f
         }
 }
 
-// joins the parts of a split key axis, in split order: a wave per row
+// joins the parts of a split key axis, in split order: a thread per four values of a row
 template <int T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnFwd<T> a) {
     const AttnShape& s = a.s;
-    const int lane = threadIdx.x & 63, rows = s.nq * s.group;
-    const int64_t n = (int64_t)s.batch * s.kv_heads * rows, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int rows = s.nq * s.group, quads = (s.dim + 3) / 4;
+    const int64_t n = (int64_t)s.batch * s.kv_heads * rows, id = (int64_t)blockIdx.x * 256 + threadIdx.x, at = id / quads;
     if (at >= n) return;
+    const int c = (int)(id - at * quads) * 4, left = min(4, s.dim - c);
     const int bh = (int)(at / rows), row = (int)(at - (int64_t)bh * rows), b = bh / s.kv_heads, hk = bh - b * s.kv_heads;
     float top = -INFINITY;
     for (int i = 0; i < a.splits; ++i) top = fmaxf(top, a.part_l[i * n + at]);
     const float use = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    for (int i = 0; i < a.splits; ++i) sum += exp2_fast(a.part_l[i * n + at] - use);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (a.lse && lane == 0) a.lse[at] = sum > 0.f ? use + log2f(sum) : INFINITY;
-    const int i0 = row_point(s, row);
-    typename Num<T>::type* o = a.out + (((int64_t)b * s.nq + i0) * s.heads + hk * s.group + row - i0 * s.group) * s.dim;
-    for (int c = lane; c < s.dim; c += 64) {
-        float v = 0.f;
-        for (int i = 0; i < a.splits; ++i) v = fmaf(exp2_fast(a.part_l[i * n + at] - use) * inv, a.part_o[(i * n + at) * s.dim + c], v);
-        store_value<T>(o + c, v);
+    float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < a.splits; ++i) {
+        const float w = exp2_fast(a.part_l[i * n + at] - use);
+        const float* p = a.part_o + (i * n + at) * s.dim + c;
+        sum += w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < left) v[e] = fmaf(w, p[e], v[e]);
     }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (a.lse && c == 0) a.lse[at] = sum > 0.f ? use + log2f(sum) : INFINITY;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= inv;
+    const int i0 = row_point(s, row);
+    store4<T>(a.out + (((int64_t)b * s.nq + i0) * s.heads + hk * s.group + row - i0 * s.group) * s.dim + c, v, left);
 }
 
 // Rows of a workgroup: 128 (four waves share every key tile), or 32 when there are no more rows than that per key head (single tokens).
@@ -223,10 +231,10 @@ static AttnPlan attn_plan(int dtype, int batch, int nq, int nk, int heads, int k
     return p;
 }
 
-template <int T, int W>
+template <int T, int W, int KS>
 static int attn_fwd_launch(const AttnFwd<T>& a, int waves, int64_t blocks, hipStream_t st) {
-    if (waves == 1) attn_fwd_kernel<T, W, 1><<<(unsigned)blocks, 64, 0, st>>>(a);
-    else attn_fwd_kernel<T, W, 4><<<(unsigned)blocks, 256, 0, st>>>(a);
+    if (waves == 1) attn_fwd_kernel<T, W, KS, 1><<<(unsigned)blocks, 64, 0, st>>>(a);
+    else attn_fwd_kernel<T, W, KS, 4><<<(unsigned)blocks, 256, 0, st>>>(a);
     EQ_CHECK_LAUNCH("attention_forward");
     return 0;
 }
@@ -248,10 +256,9 @@ static int attn_fwd(const equigspr_attention* d, const AttnShape& s, void* out, 
     a.part_o = work + (p.splits > 1 ? (p.splits * n + 3) / 4 * 4 : 0);
     const int64_t blocks = (int64_t)p.row_tiles * p.splits * s.batch * s.kv_heads;
     EQ_CHECK_ARG(blocks < (1 << 24), EQUIGSPR_ENOTSUP, "attention: %lld workgroups are more than one launch takes", (long long)blocks);
-    int rc = s.dim <= 32 ? attn_fwd_launch<T, 32>(a, p.waves, blocks, st) : s.dim <= 64 ? attn_fwd_launch<T, 64>(a, p.waves, blocks, st)
-                                                                                       : attn_fwd_launch<T, 128>(a, p.waves, blocks, st);
+    const int rc = EQ_ATTN_BY_DIM(attn_fwd_launch, s.dim, a, p.waves, blocks, st);
     if (rc || p.splits == 1) return rc;
-    attn_join_kernel<T><<<(unsigned)ceil_div(n, 4), 256, 0, st>>>(a);
+    attn_join_kernel<T><<<(unsigned)ceil_div(n * ((s.dim + 3) / 4), 256), 256, 0, st>>>(a);
     EQ_CHECK_LAUNCH("attention_forward (join)");
     return 0;
 }

@@ -11,7 +11,7 @@
 
 namespace eq {
 
-constexpr int kAmaxBlocks = 256;
+constexpr int kAmaxBlocks = 1024;
 
 template <int T>
 struct AttnBwd {
@@ -36,20 +36,24 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(AttnBwd<T> a) {
     const AttnShape& s = a.s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float mg = 0.f, mv = 0.f;
-    const int64_t ng = (int64_t)s.batch * s.nq * s.heads, nv = (int64_t)s.batch * s.nk * s.kv_heads;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < ng; r += kAmaxBlocks * 4) {
-        const int64_t bi = r / s.heads;
-        const int h = (int)(r - bi * s.heads), b = (int)(bi / s.nq), i = (int)(bi - (int64_t)b * s.nq);
-        if (i >= attn_len(s.q_lens, b, s.nq)) continue;
-        const typename Num<T>::type* p = a.g.p + b * a.g.sb + i * a.g.sn + h * a.g.sh;
-        for (int c = lane; c < s.dim; c += 64) mg = fmaxf(mg, fabsf((float)p[c]));
+    const int chunks = (s.dim + 7) / 8;
+    auto most = [&](float& m, const typename Num<T>::type* row, int c) {
+        const Raw8<T> r = load8<T>(row, 8 * c, s.dim);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(raw_float<T>(r, i)));
+    };
+    // a thread per chunk of eight values
+    const int64_t ng = (int64_t)s.batch * s.nq, nv = (int64_t)s.batch * s.nk;
+    const int per_g = s.heads * chunks, per_v = s.kv_heads * chunks;
+    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < ng * per_g; id += kAmaxBlocks * 256) {
+        const int64_t pt = id / per_g;
+        const int hc = (int)(id - pt * per_g), h = hc / chunks, b = (int)(pt / s.nq), i = (int)(pt - (int64_t)b * s.nq);
+        if (i < attn_len(s.q_lens, b, s.nq)) most(mg, a.g.p + b * a.g.sb + i * a.g.sn + h * a.g.sh, hc - h * chunks);
     }
-    for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < nv; r += kAmaxBlocks * 4) {
-        const int64_t bi = r / s.kv_heads;
-        const int h = (int)(r - bi * s.kv_heads), b = (int)(bi / s.nk), j = (int)(bi - (int64_t)b * s.nk);
-        if (j >= attn_len(s.kv_lens, b, s.nk) || (s.key_mask && !s.key_mask[b * s.mask_stride + j])) continue;
-        const typename Num<T>::type* p = key_row(a.v, b, h, j);
-        for (int c = lane; c < s.dim; c += 64) mv = fmaxf(mv, fabsf((float)p[c]));
+    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < nv * per_v; id += kAmaxBlocks * 256) {
+        const int64_t pt = id / per_v;
+        const int hc = (int)(id - pt * per_v), h = hc / chunks, b = (int)(pt / s.nk), j = (int)(pt - (int64_t)b * s.nk);
+        if (j < attn_len(s.kv_lens, b, s.nk) && (!s.key_mask || s.key_mask[b * s.mask_stride + j])) most(mv, key_row(a.v, b, h, j), hc - h * chunks);
     }
     __shared__ float part[2][4];
     for (int o = 32; o; o >>= 1) { mg = fmaxf(mg, __shfl_xor(mg, o)); mv = fmaxf(mv, __shfl_xor(mv, o)); }
@@ -79,10 +83,10 @@ __device__ __forceinline__ float attn_grad_scale(const AttnBwd<T>& a) {
 
 constexpr int kBwdWaves = 4;                  // waves of a workgroup: each owns 32 rows (keys), all share the staged tiles
 
-template <int T, int W>
+template <int T, int W, int KS>
 __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_kernel(AttnBwd<T> a) {
     constexpr int KT = attn_bwd_tile<T, W>(), NT = kBwdWaves * 64, ROWS = kBwdWaves * 32, NP = Num<T>::planes;
-    constexpr int KS = W / 16, DB = W / 32, KB = KT / 32;
+    constexpr int DB = (KS + 1) / 2, KB = KT / 32;
     __shared__ __attribute__((aligned(16))) short tile_k[NP * Tile<W>::size(KT)];
     __shared__ __attribute__((aligned(16))) short tile_v[NP * Tile<W>::size(KT)];
     __shared__ __attribute__((aligned(16))) float hidden[KT];
@@ -161,11 +165,13 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_ker
             pf32x16 sc, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) sc[r] = dp[r] = 0.f;
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 mma<T>(sc, tile_rows<T, W, KT>(tile_k, kb * 32, ks, lane), q[ks]);
                 mma<T>(dp, tile_rows<T, W, KT>(tile_v, kb * 32, ks, lane), g[ks]);
             }
+            __builtin_amdgcn_s_setprio(0);
             if (edge) {
                 asm volatile("");                         // a branch: as selects this would be a third of the tile's arithmetic
 #pragma unroll
@@ -207,10 +213,10 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_ker
         }
 }
 
-template <int T, int W>
+template <int T, int W, int KS>
 __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dkv_kernel(AttnBwd<T> a) {
     constexpr int RT = attn_bwd_tile<T, W>(), NT = kBwdWaves * 64, KEYS = kBwdWaves * 32, NP = Num<T>::planes;
-    constexpr int KS = W / 16, DB = W / 32, RB = RT / 32;
+    constexpr int DB = (KS + 1) / 2, RB = RT / 32;
     constexpr float kShift = T == kF16 ? 10.f : 0.f;
     __shared__ __attribute__((aligned(16))) short tile_q[NP * Tile<W>::size(RT)];
     __shared__ __attribute__((aligned(16))) short tile_g[NP * Tile<W>::size(RT)];
@@ -289,6 +295,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dkv_ke
             pf32x16 sc, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) sc[r] = dp[r] = 0.f;
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 mma<T>(sc, tile_rows<T, W, RT>(tile_q, rb * 32, ks, lane), k[ks]);
@@ -308,6 +315,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dkv_ke
                     dp[4 * gr + i] = p * (dp[4 * gr + i] - del[i]) * fs;
                 }
             }
+            __builtin_amdgcn_s_setprio(0);
             if (edge) {
                 asm volatile("");                         // a branch, see above
 #pragma unroll
@@ -397,7 +405,7 @@ static AttnBwdPlan attn_bwd_plan(const AttnShape& s) {
     return p;
 }
 
-template <int T, int W>
+template <int T, int W, int KS>
 static int attn_bwd_launch(const AttnBwd<T>& a, hipStream_t st) {
     const AttnShape& s = a.s;
     const int64_t heads = (int64_t)s.batch * s.kv_heads;
@@ -408,7 +416,7 @@ static int attn_bwd_launch(const AttnBwd<T>& a, hipStream_t st) {
         EQ_CHECK_LAUNCH("attention_backward (range)");
     }
     if (bq) {
-        attn_dq_kernel<T, W><<<(unsigned)bq, kBwdWaves * 64, 0, st>>>(a);
+        attn_dq_kernel<T, W, KS><<<(unsigned)bq, kBwdWaves * 64, 0, st>>>(a);
         EQ_CHECK_LAUNCH("attention_backward (rows)");
         if (a.key_splits > 1 && a.gq) {
             const int64_t n = heads * s.nq * s.group * s.dim, blocks = ceil_div(n, 1024);
@@ -417,7 +425,7 @@ static int attn_bwd_launch(const AttnBwd<T>& a, hipStream_t st) {
         }
     }
     if (bk && (a.gk || a.gv)) {
-        attn_dkv_kernel<T, W><<<(unsigned)bk, kBwdWaves * 64, 0, st>>>(a);
+        attn_dkv_kernel<T, W, KS><<<(unsigned)bk, kBwdWaves * 64, 0, st>>>(a);
         EQ_CHECK_LAUNCH("attention_backward (keys)");
         if (a.row_splits > 1) {
             const int64_t n = heads * s.nk * s.dim, blocks = ceil_div(n, 1024);
@@ -448,7 +456,7 @@ static int attn_bwd(const equigspr_attention* d, const AttnShape& s, const void*
     a.part_v = a.part_k + p.parts_k;
     a.row_tiles = p.row_tiles; a.key_tiles = p.key_tiles; a.key_splits = p.key_splits; a.split_keys = p.split_keys; a.row_splits = p.row_splits;
     a.gq = (E*)gq; a.gk = (E*)gk; a.gv = (E*)gv;
-    return s.dim <= 32 ? attn_bwd_launch<T, 32>(a, st) : s.dim <= 64 ? attn_bwd_launch<T, 64>(a, st) : attn_bwd_launch<T, 128>(a, st);
+    return EQ_ATTN_BY_DIM(attn_bwd_launch, s.dim, a, st);
 }
 
 }  // namespace eq

@@ -134,6 +134,11 @@ constexpr int kAttnMaxDim = 128;
 template <int T, int W> constexpr int attn_tile() { return T == kF32 && W > 32 ? 32 : 64; }
 
 // ---- host side
+// f<T, W, KS>: the head dim in steps of 16, in tiles of 32, 64 or 128 columns (dims up to 16 and up to 96 skip the empty steps)
+#define EQ_ATTN_BY_DIM(f, dim, ...)                                                                               \
+    ((dim) <= 16 ? f<T, 32, 1>(__VA_ARGS__) : (dim) <= 32 ? f<T, 32, 2>(__VA_ARGS__) : (dim) <= 64 ? f<T, 64, 4>(__VA_ARGS__) \
+     : (dim) <= 96 ? f<T, 128, 6>(__VA_ARGS__) : f<T, 128, 8>(__VA_ARGS__))
+
 template <int T>
 static inline AttnTensor<T> attn_tensor(const equigspr_attention_tensor& t, int dim) {
     using E = typename Num<T>::type;
