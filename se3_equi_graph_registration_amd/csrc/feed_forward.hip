@@ -56,34 +56,53 @@ __device__ __forceinline__ void activate(int act, float z, float& a, float& d) {
     }
 }
 
-// tile of 128 x 128 outputs, four waves of 64 x 64
-constexpr int kFfTile = 128;
-template <int T> constexpr int ff_k_tile() { return T == kF32 ? 32 : 64; }
+// Two output tiles.  Large: 256 x 256, eight waves of 128 x 64, two buffers of 64 k (16-bit types): per step of 16 a wave reads six
+// operands for eight products, a compute unit's LDS keeps up with its matrix pipes, and memory is read half as often as by 128 x 128.
+// Small: 128 x 128, four waves of 64 x 64, one buffer; for outputs that would leave compute units idle, and for the three planes of fp32.
+template <int T, bool kLarge>
+struct FfShapeOf {
+    static_assert(!kLarge || T != kF32, "three planes do not fit the large tile");
+    static constexpr int kBK = T == kF32 ? 32 : 64, kMB = kLarge ? 4 : 2, kWavesN = kLarge ? 4 : 2, kWaves = 2 * kWavesN;
+    static constexpr int kBM = 2 * kMB * 32, kBN = kWavesN * 64, kThreads = kWaves * 64, kBuffers = kLarge ? 2 : 1;
+};
 
-// kAcross: the operand's contraction runs across its rows in memory (tile [k][m]) instead of along them (tile [m][k])
-template <int T, bool kAcross>
+// kAcross: the operand's contraction runs across its rows in memory (tile [k][outer]) instead of along them (tile [outer][k])
+template <int T, bool kAcross, int kOuter, int BK, int NT>
 struct FfTile {
-    static constexpr int BK = ff_k_tile<T>(), W = kAcross ? kFfTile : BK, ROWS = kAcross ? BK : kFfTile;
-    static constexpr int kPlane = Tile<W>::size(ROWS), kPer = ROWS * W / 8 / 256;
+    using E = typename Num<T>::type;
+    static constexpr int W = kAcross ? kOuter : BK, ROWS = kAcross ? BK : kOuter;
+    static constexpr int kPlane = Tile<W>::size(ROWS), kPer = ROWS * W / 8 / NT;
+    static_assert(kPer * NT * 8 == ROWS * W, "whole chunks per thread");
     Raw8<T> raw[kPer];
-    // outer0: first output row / column of the tile; k0: first contraction index; k_end bounds it
+    // outer0: first output row / column of the tile; k0: first contraction index; k_end bounds it.  outer_row(r, clamp): the memory row of
+    // output r (along): null where there is none, or the last one if clamp (its products are never stored)
     template <class F>
     __device__ __forceinline__ void load(const FfOperand<T>& o, int outer0, int k0, int k_end, F outer_row) {
+        const bool whole = k0 + BK <= k_end && (!kAcross || outer0 + W <= o.len);
+        if (whole) {
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) {
-            const int id = threadIdx.x + u * 256, r = id / (W / 8), c = id % (W / 8) * 8;
-            if constexpr (kAcross) {
-                raw[u] = k0 + r < k_end ? load8<T>(o.row(k0 + r) + outer0, c, o.len - outer0) : raw_zero<T>();
-            } else {
-                const typename Num<T>::type* row = outer_row(r);
-                raw[u] = row ? load8<T>(row + k0, c, k_end - k0) : raw_zero<T>();
+            for (int u = 0; u < kPer; ++u) {
+                const int id = threadIdx.x + u * NT, r = id / (W / 8), c = id % (W / 8) * 8;
+                const E* p = kAcross ? o.row(k0 + r) + outer0 + c : outer_row(r, true) + k0 + c;
+                raw[u] = load8<T>(p, 0, 8);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < kPer; ++u) {
+                const int id = threadIdx.x + u * NT, r = id / (W / 8), c = id % (W / 8) * 8;
+                if constexpr (kAcross) {
+                    raw[u] = k0 + r < k_end ? load8<T>(o.row(k0 + r) + outer0, c, o.len - outer0) : raw_zero<T>();
+                } else {
+                    const E* row = outer_row(r, false);
+                    raw[u] = row ? load8<T>(row + k0, c, k_end - k0) : raw_zero<T>();
+                }
             }
         }
     }
     __device__ __forceinline__ void store(short* tile) const {
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
-            const int id = threadIdx.x + u * 256;
+            const int id = threadIdx.x + u * NT;
             const Op8<T> o = planes_of<T>(raw[u]);
 #pragma unroll
             for (int p = 0; p < Num<T>::planes; ++p) *reinterpret_cast<s16x8*>(tile + p * kPlane + Tile<W>::at(id / (W / 8), id % (W / 8))) = o.p[p];
@@ -106,125 +125,167 @@ struct FfTile {
     }
 };
 
-template <int T, bool kAcrossA, bool kAcrossB, int kEpi>
-__global__ __launch_bounds__(256) void ff_product_kernel(FfArgs<T> g) {
-    using TA = FfTile<T, kAcrossA>;
-    using TB = FfTile<T, kAcrossB>;
-    constexpr int BK = ff_k_tile<T>(), NP = Num<T>::planes, TN = kEpi == kGate ? kFfTile / 2 : kFfTile;
-    __shared__ __attribute__((aligned(16))) short tile_a[NP * TA::kPlane];
-    __shared__ __attribute__((aligned(16))) short tile_b[NP * TB::kPlane];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wm = wave >> 1, wn = wave & 1;
-    int id = xcd_block(blockIdx.x, gridDim.x);
-    const int tm = id % g.tiles_m;
-    id /= g.tiles_m;
-    const int tn = id % g.tiles_n, cut = id / g.tiles_n;
-    const int m0 = tm * kFfTile, n0 = tn * TN, k_begin = cut * g.cut_k, k_end = min(g.k, k_begin + g.cut_k);
-    auto row_a = [&](int r) { return m0 + r < g.a.rows ? g.a.row(m0 + r) : nullptr; };
-    auto row_b = [&](int r) -> const typename Num<T>::type* {
-        if constexpr (kEpi == kGate) {            // tile rows 0..63: gate columns, 64..127: the same columns of the other projection
-            const int c = n0 + (r & 63);
-            return c < g.n ? (r < 64 ? g.b.p : g.b.q) + c * g.b.ld : nullptr;
+template <int T, bool kAcrossA, bool kAcrossB, int kEpi, bool kLarge>
+__global__ __launch_bounds__((FfShapeOf<T, kLarge>::kThreads), 2) void ff_product_kernel(FfArgs<T> g) {
+    using S = FfShapeOf<T, kLarge>;
+    using E = typename Num<T>::type;
+    constexpr int BK = S::kBK, BM = S::kBM, BN = S::kBN, MB = S::kMB, NP = Num<T>::planes, TN = kEpi == kGate ? BN / 2 : BN, NBUF = S::kBuffers;
+    using TA = FfTile<T, kAcrossA, BM, BK, S::kThreads>;
+    using TB = FfTile<T, kAcrossB, BN, BK, S::kThreads>;
+    // the staged tiles; at the end each wave turns 32 x 64 results at a time from matrix layout to rows in its own part
+    constexpr int kTileA = NP * TA::kPlane, kTileB = NP * TB::kPlane, kOutStride = 68, kOutFloats = 32 * kOutStride;
+    __shared__ __attribute__((aligned(16))) short lds[NBUF * (kTileA + kTileB)];
+    static_assert(sizeof(lds) >= sizeof(float) * kOutFloats * S::kWaves, "room for the results");
+    auto tile_a = [&](int buf) { return lds + buf * kTileA; };
+    auto tile_b = [&](int buf) { return lds + NBUF * kTileA + buf * kTileB; };
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wm = wave / S::kWavesN, wn = wave % S::kWavesN;
+    // neighbours on an XCD take 8 row tiles by some column tiles: both operands' panels are shared in its L2
+    const int id = xcd_block(blockIdx.x, gridDim.x), per_cut = g.tiles_m * g.tiles_n, cut = id / per_cut, rest = id - cut * per_cut;
+    const int band = rest / (8 * g.tiles_n), in_band = rest - band * 8 * g.tiles_n, band_rows = min(8, g.tiles_m - 8 * band);
+    const int tm = 8 * band + in_band % band_rows, tn = in_band / band_rows;
+    const int m0 = tm * BM, n0 = tn * TN, k_begin = cut * g.cut_k, k_end = min(g.k, k_begin + g.cut_k);
+    auto row_a = [&](int r, bool clamp) -> const E* {
+        const int m = m0 + r;
+        return clamp ? g.a.row(min(m, g.a.rows - 1)) : m < g.a.rows ? g.a.row(m) : nullptr;
+    };
+    auto row_b = [&](int r, bool clamp) -> const E* {
+        if constexpr (kEpi == kGate) {            // the tile's first half: columns of one projection; its second half: the same of the other
+            int c = n0 + r % TN;
+            if (clamp) c = min(c, g.n - 1);
+            return c < g.n ? (r < TN ? g.b.p : g.b.q) + c * g.b.ld : nullptr;
         } else {
-            return n0 + r < g.b.rows ? g.b.row(n0 + r) : nullptr;
+            const int n = n0 + r;
+            return clamp ? g.b.row(min(n, g.b.rows - 1)) : n < g.b.rows ? g.b.row(n) : nullptr;
         }
     };
     // acc[i][j]: C tile with the output's columns in the registers (block j) and its rows in the lanes (block i)
-    pf32x16 acc[2][2];
+    pf32x16 acc[MB][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MB; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    const int om[2] = {wm * 64, wm * 64 + 32};
-    const int on[2] = {kEpi == kGate ? wn * 32 : wn * 64, kEpi == kGate ? 64 + wn * 32 : wn * 64 + 32};
+    const int om = wm * MB * 32;
+    const int on[2] = {kEpi == kGate ? wn * 32 : wn * 64, kEpi == kGate ? TN + wn * 32 : wn * 64 + 32};
     TA sa;
     TB sb;
-    sa.load(g.a, m0, k_begin, k_end, row_a);
-    sb.load(g.b, n0, k_begin, k_end, row_b);
-    for (int k0 = k_begin; k0 < k_end; k0 += BK) {
-        __syncthreads();
-        sa.store(tile_a);
-        sb.store(tile_b);
-        __syncthreads();
-        if (k0 + BK < k_end) {
-            sa.load(g.a, m0, k0 + BK, k_end, row_a);
-            sb.load(g.b, n0, k0 + BK, k_end, row_b);
-        }
+    auto multiply = [&](int buf, auto midway) {
 #pragma unroll
         for (int ks = 0; ks < BK / 16; ++ks) {
-            Op8<T> pa[2], pb[2];
+            Op8<T> pa[MB], pb[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                pa[i] = TA::operand(tile_a, om[i], ks, lane);
-                pb[i] = TB::operand(tile_b, on[i], ks, lane);
-            }
+            for (int j = 0; j < 2; ++j) pb[j] = TB::operand(tile_b(buf), on[j], ks, lane);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < MB; ++i) pa[i] = TA::operand(tile_a(buf), om + 32 * i, ks, lane);
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) mma<T>(acc[i][j], pb[j], pa[i]);
+            if (ks == BK / 32 - 1) midway();
+        }
+    };
+    sa.load(g.a, m0, k_begin, k_end, row_a);
+    sb.load(g.b, n0, k_begin, k_end, row_b);
+    if constexpr (NBUF == 2) {
+        sa.store(tile_a(0));
+        sb.store(tile_b(0));
+        int buf = 0;
+        for (int k0 = k_begin; k0 < k_end; k0 += BK, buf ^= 1) {
+            const bool more = k0 + BK < k_end;
+            if (more) {
+                sa.load(g.a, m0, k0 + BK, k_end, row_a);
+                sb.load(g.b, n0, k0 + BK, k_end, row_b);
+            }
+            __syncthreads();                      // this buffer is written, the other one has been read
+            multiply(buf, [&] {                   // halfway: the loads have arrived, and the waves meet next with nothing left to write
+                if (more) {
+                    sa.store(tile_a(buf ^ 1));
+                    sb.store(tile_b(buf ^ 1));
+                }
+            });
+        }
+    } else {
+        for (int k0 = k_begin; k0 < k_end; k0 += BK) {
+            __syncthreads();
+            sa.store(tile_a(0));
+            sb.store(tile_b(0));
+            __syncthreads();
+            if (k0 + BK < k_end) {
+                sa.load(g.a, m0, k0 + BK, k_end, row_a);
+                sb.load(g.b, n0, k0 + BK, k_end, row_b);
+            }
+            multiply(0, [] {});
         }
     }
-    using E = typename Num<T>::type;
+    __syncthreads();                              // the last tiles have been read
+    float* const out = reinterpret_cast<float*>(lds) + wave * kOutFloats;
+    constexpr int kCols = kEpi == kGate ? 32 : 64, kLanes = kCols / 8, kRows = 64 / kLanes;      // columns, lanes per row, rows of a step
+    const int col = n0 + (kEpi == kGate ? wn * 32 : wn * 64) + lane % kLanes * 8, left = g.n - col;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int row = m0 + om[i] + (lane & 31);
-        if (row >= g.m) continue;
-        if constexpr (kEpi == kGate) {
+    for (int i = 0; i < MB; ++i) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int col = n0 + on[0] + 8 * q + 4 * half, left = g.n - col;
-                if (left <= 0) continue;
-                float z[4], u[4], h[4];
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    z[e] = acc[i][0][4 * q + e] + (g.bias && e < left ? (float)g.bias[col + e] : 0.f);
-                    u[e] = acc[i][1][4 * q + e] + (g.bias2 && e < left ? (float)g.bias2[col + e] : 0.f);
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<pf32x4*>(out + (lane & 31) * kOutStride + 32 * j + 8 * q + 4 * half) =
+                    (pf32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+        for (int r0 = 0; r0 < 32; r0 += kRows) {
+            const int r = r0 + lane / kLanes, row = m0 + om + 32 * i + r;
+            float v[8], z[8], u[8];
+            const float* src = out + r * kOutStride + lane % kLanes * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = src[e];
+            if (row >= g.m || left <= 0) continue;
+            if constexpr (kEpi == kGate) {
+                float h[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { z[e] = 0.f; u[e] = 0.f; }
+                if (g.bias) load8f<T>(g.bias + col, left, z);
+                if (g.bias2) load8f<T>(g.bias2 + col, left, u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
                     float a, d;
+                    z[e] += v[e];
+                    u[e] += src[32 + e];
                     activate(g.act, z[e], a, d);
                     h[e] = a * u[e];
                 }
-                store4<T>(g.c + (int64_t)row * g.n + col, h, left);
+                store8<T>(g.c + (int64_t)row * g.n + col, h, left);
                 if (g.zu) {
-                    store4<T>(g.zu + (int64_t)row * 2 * g.n + col, z, left);
-                    store4<T>(g.zu + (int64_t)row * 2 * g.n + g.n + col, u, left);
+                    store8<T>(g.zu + (int64_t)row * 2 * g.n + col, z, left);
+                    store8<T>(g.zu + (int64_t)row * 2 * g.n + g.n + col, u, left);
                 }
+            } else if constexpr (kEpi == kGrad) {
+                const int64_t at = (int64_t)row * 2 * g.n + col;
+                float h[8];
+                load8f<T>(g.zu + at, left, z);
+                load8f<T>(g.zu + at + g.n, left, u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float a, d;
+                    activate(g.act, z[e], a, d);
+                    h[e] = a * u[e];
+                    z[e] = v[e] * u[e] * d;
+                    u[e] = v[e] * a;
+                }
+                store8<T>(g.dzu + at, z, left);
+                store8<T>(g.dzu + at + g.n, u, left);
+                store8<T>(g.h + (int64_t)row * g.n + col, h, left);
+            } else if (g.cuts > 1) {
+                store8<kF32>(g.part + ((int64_t)cut * g.m + row) * g.n + col, v, left);
+            } else {
+                if (g.bias) {
+                    load8f<T>(g.bias + col, left, z);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += z[e];
+                }
+                store8<T>(g.c + (int64_t)row * g.n + col, v, left);
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int col = n0 + on[j] + 8 * q + 4 * half, left = g.n - col;
-                    if (left <= 0) continue;
-                    float v[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
-                    if constexpr (kEpi == kGrad) {
-                        const E* pz = g.zu + (int64_t)row * 2 * g.n + col;
-                        float dz[4], du[4], h[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float z = e < left ? (float)pz[e] : 0.f, u = e < left ? (float)pz[g.n + e] : 0.f;
-                            float a, d;
-                            activate(g.act, z, a, d);
-                            h[e] = a * u;
-                            dz[e] = v[e] * u * d;
-                            du[e] = v[e] * a;
-                        }
-                        store4<T>(g.dzu + (int64_t)row * 2 * g.n + col, dz, left);
-                        store4<T>(g.dzu + (int64_t)row * 2 * g.n + g.n + col, du, left);
-                        store4<T>(g.h + (int64_t)row * g.n + col, h, left);
-                    } else if (g.cuts > 1) {
-                        store4<kF32>(g.part + ((int64_t)cut * g.m + row) * g.n + col, v, left);
-                    } else {
-                        if (g.bias)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) v[e] += e < left ? (float)g.bias[col + e] : 0.f;
-                        store4<T>(g.c + (int64_t)row * g.n + col, v, left);
-                    }
-                }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
@@ -262,31 +323,44 @@ __global__ __launch_bounds__(256) void ff_columns_sum_kernel(const float* part, 
 
 struct FfShape { int rows, width, hidden, out; };
 
-// Cuts of a contraction: when the output's tiles leave compute units idle, into parts of at least four k tiles.
-static int ff_cuts(int64_t tiles, int k, int bk) {
-    if (tiles >= 256) return 1;
-    const int64_t most = k / (4 * bk), want = 512 / (tiles > 0 ? tiles : 1);
-    const int64_t c = want < most ? want : most;
-    return c > 1 ? (int)c : 1;
+// Tile and cuts of a product.  The large tile when it gives at least half the compute units a workgroup; a contraction is cut when the
+// tiles leave compute units idle, into parts of at least 256 (large: 1024) k.
+struct FfPlan { bool large; int tiles_m, tiles_n, cuts, cut_k; };
+static FfPlan ff_plan(int dtype, bool gate, bool can_cut, int m, int n, int k) {
+    FfPlan p;
+    const int columns = gate ? 2 * n : n;
+    p.large = dtype != kF32 && (int64_t)ceil_div(m, 256) * ceil_div(columns, 256) >= 128;
+    const int side = p.large ? 256 : 128, bk = dtype == kF32 ? 32 : 64;
+    p.tiles_m = ceil_div(m, side);
+    p.tiles_n = ceil_div(n, gate ? side / 2 : side);
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, full = p.large ? 256 : 512, least = p.large ? 1024 : 256;
+    int64_t c = 1;
+    if (can_cut && tiles > 0 && tiles <= full / 2) {
+        c = full / tiles;
+        if (c > k / least) c = k / least;
+        if (c < 1) c = 1;
+    }
+    p.cut_k = k > 0 ? ceil_div(ceil_div(k, c), bk) * bk : bk;
+    p.cuts = k > 0 ? ceil_div(k, p.cut_k) : 1;
+    return p;
 }
-static int64_t ff_part_size(int m, int n, int k, int bk) {
-    const int64_t c = ff_cuts((int64_t)ceil_div(m, kFfTile) * ceil_div(n, kFfTile), k, bk);
-    return c > 1 ? c * m * n : 0;
+static int64_t ff_part_size(int dtype, int m, int n, int k) {
+    const FfPlan p = ff_plan(dtype, false, true, m, n, k);
+    return p.cuts > 1 ? (int64_t)p.cuts * m * n : 0;
 }
 constexpr int kFfRun = 256;                   // rows of a run of a column sum
 
 template <int T, bool kAcrossA, bool kAcrossB, int kEpi>
 static int ff_product(FfArgs<T> g, hipStream_t st, const char* what) {
-    constexpr int BK = ff_k_tile<T>(), TN = kEpi == kGate ? kFfTile / 2 : kFfTile;
-    g.tiles_m = ceil_div(g.m, kFfTile);
-    g.tiles_n = ceil_div(g.n, TN);
-    g.cuts = kEpi == kPlain ? ff_cuts((int64_t)g.tiles_m * g.tiles_n, g.k, BK) : 1;
-    g.cut_k = ceil_div(ceil_div(g.k, g.cuts), BK) * BK;
-    g.cuts = ceil_div(g.k, g.cut_k);
+    const FfPlan p = ff_plan(T, kEpi == kGate, kEpi == kPlain, g.m, g.n, g.k);
+    g.tiles_m = p.tiles_m; g.tiles_n = p.tiles_n; g.cuts = p.cuts; g.cut_k = p.cut_k;
     const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.cuts;
     if (blocks == 0) return 0;
-    EQ_CHECK_ARG(blocks < (1 << 24), EQUIGSPR_ENOTSUP, "%s: more workgroups than one launch takes", what);
-    ff_product_kernel<T, kAcrossA, kAcrossB, kEpi><<<(unsigned)blocks, 256, 0, st>>>(g);
+    EQ_CHECK_ARG(blocks < (1 << 23), EQUIGSPR_ENOTSUP, "%s: more workgroups than one launch takes", what);
+    if constexpr (T != kF32) {
+        if (p.large) ff_product_kernel<T, kAcrossA, kAcrossB, kEpi, true><<<(unsigned)blocks, 512, 0, st>>>(g);
+    }
+    if (!p.large) ff_product_kernel<T, kAcrossA, kAcrossB, kEpi, false><<<(unsigned)blocks, 256, 0, st>>>(g);
     EQ_CHECK_LAUNCH(what);
     if (g.cuts > 1) {
         const int64_t n = ceil_div((int64_t)g.m * g.n, 256);
@@ -392,7 +466,7 @@ static int ff_check(const equigspr_gated_feed_forward* d) {
 
 extern "C" int64_t equigspr_gated_feed_forward_work_size(const equigspr_gated_feed_forward* d) {
     if (eq::ff_check(d) != 0) return -1;
-    return eq::ff_part_size(d->rows, d->out, d->hidden, d->dtype == EQUIGSPR_F32 ? eq::ff_k_tile<eq::kF32>() : eq::ff_k_tile<eq::kBF16>());
+    return eq::ff_part_size(d->dtype, d->rows, d->out, d->hidden);
 }
 
 extern "C" int equigspr_gated_feed_forward_forward(const equigspr_gated_feed_forward* d, void* y, void* h, void* zu, float* work, void* stream) {
@@ -409,9 +483,8 @@ extern "C" int equigspr_gated_feed_forward_forward(const equigspr_gated_feed_for
 
 extern "C" int64_t equigspr_gated_feed_forward_backward_work_size(const equigspr_gated_feed_forward* d) {
     if (eq::ff_check(d) != 0) return -1;
-    const int bk = d->dtype == EQUIGSPR_F32 ? eq::ff_k_tile<eq::kF32>() : eq::ff_k_tile<eq::kBF16>();
-    int64_t n = eq::ff_part_size(d->rows, d->width, 2 * d->hidden, bk);
-    const int64_t up = eq::ff_part_size(2 * d->hidden, d->width, d->rows, bk), down = eq::ff_part_size(d->out, d->hidden, d->rows, bk);
+    int64_t n = eq::ff_part_size(d->dtype, d->rows, d->width, 2 * d->hidden);
+    const int64_t up = eq::ff_part_size(d->dtype, 2 * d->hidden, d->width, d->rows), down = eq::ff_part_size(d->dtype, d->out, d->hidden, d->rows);
     const int64_t widest = 2 * d->hidden > d->out ? 2 * d->hidden : d->out, sums = (int64_t)eq::ceil_div(d->rows, eq::kFfRun) * widest;
     n = up > n ? up : n;
     n = down > n ? down : n;

@@ -157,8 +157,8 @@ __device__ __forceinline__ Raw8<T> load8(const typename Num<T>::type* row, int c
 // address register per k-step: in the kernels' keys' gradients at W = 128 that was the difference between one and two waves per SIMD.)
 template <int W>
 struct Tile {
-    static_assert(W == 32 || W == 64 || W == 128, "tile width");
-    static constexpr int kStride = W == 32 ? 40 : W == 64 ? 72 : 152;
+    static_assert(W == 32 || W == 64 || W == 128 || W == 256, "tile width");
+    static constexpr int kStride = W == 32 ? 40 : W == 64 ? 72 : W == 128 ? 152 : 280;
     // values of a tile of `rows` rows
     __host__ __device__ static constexpr int size(int rows) { return rows * kStride; }
     // offset (in 16-bit values) of chunk c of row r
@@ -185,6 +185,25 @@ __device__ __forceinline__ int xcd_block(int id, int n) {
 template <int T>
 __device__ __forceinline__ void store_value(typename Num<T>::type* p, float v) { *p = (typename Num<T>::type)v; }
 
+// the first n of four consecutive values, the rest zero
+template <int T>
+__device__ __forceinline__ void load4(const typename Num<T>::type* p, int n, float (&v)[4]) {
+    if (n >= 4) {
+        if constexpr (T == kF32) {
+            const pf32x4 r = *reinterpret_cast<const pf32x4_u*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = r[i];
+        } else {
+            const s16x4 r = *reinterpret_cast<const s16x4_u*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = (float)__builtin_bit_cast(typename Num<T>::type, (short)r[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+    }
+}
+
 // the first n of four consecutive values
 template <int T>
 __device__ __forceinline__ void store4(typename Num<T>::type* p, const float (&v)[4], int n) {
@@ -202,6 +221,35 @@ __device__ __forceinline__ void store4(typename Num<T>::type* p, const float (&v
         for (int i = 0; i < 3; ++i)
             if (i < n) store_value<T>(p + i, v[i]);
     }
+}
+
+// eight consecutive values, of which the first n exist
+template <int T>
+__device__ __forceinline__ void load8f(const typename Num<T>::type* p, int n, float (&v)[8]) {
+    const Raw8<T> r = load8<T>(p, 0, n);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = raw_float<T>(r, i);
+}
+template <int T>
+__device__ __forceinline__ void store8(typename Num<T>::type* p, const float (&v)[8], int n) {
+    if constexpr (T != kF32) {
+        if (n >= 8) {
+            u32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                unsigned o[1];
+                split2<T>(v[2 * i], v[2 * i + 1], o);
+                w[i] = o[0];
+            }
+            *reinterpret_cast<s16x8_u*>(p) = __builtin_bit_cast(s16x8, w);
+            return;
+        }
+    }
+    float a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { a[i] = v[i]; b[i] = v[4 + i]; }
+    store4<T>(p, a, n);
+    if (n > 4) store4<T>(p + 4, b, n - 4);
 }
 
 }  // namespace eq
