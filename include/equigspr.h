@@ -551,13 +551,13 @@ typedef struct equigspr_gated_feed_forward {
 typedef struct equigspr_gated_feed_forward_grads {
     void *grad_x, *grad_w_gate_up, *grad_w_down, *grad_b_gate_up, *grad_b_down;
 } equigspr_gated_feed_forward_grads;
-/* y [rows, out]; h [rows, hidden] scratch of the inputs' dtype; zu [rows, 2 * hidden] or null: both projections, kept for the backward;
+/* y [rows, out]; h [rows, hidden] (inputs' dtype): act(z) * u, kept for the backward; zu [rows, 2 * hidden] or null: both projections, likewise;
  * work: ..._work_size floats (0: may be null) */
 int64_t equigspr_gated_feed_forward_work_size(const equigspr_gated_feed_forward* desc);
 int equigspr_gated_feed_forward_forward(const equigspr_gated_feed_forward* desc, void* y, void* h, void* zu, float* work, void* stream);
-/* grad_y [rows, out] contiguous; zu as the forward wrote it; h [rows, hidden] and dzu [rows, 2 * hidden]: scratch of the inputs' dtype */
+/* grad_y [rows, out] contiguous; zu and h as the forward wrote them; dzu [rows, 2 * hidden]: scratch of the inputs' dtype */
 int64_t equigspr_gated_feed_forward_backward_work_size(const equigspr_gated_feed_forward* desc);
-int equigspr_gated_feed_forward_backward(const equigspr_gated_feed_forward* desc, const void* grad_y, const void* zu, void* h, void* dzu, float* work,
+int equigspr_gated_feed_forward_backward(const equigspr_gated_feed_forward* desc, const void* grad_y, const void* zu, const void* h, void* dzu, float* work,
                                          const equigspr_gated_feed_forward_grads* grads, void* stream);
 
 /* The residual step between two blocks, with the norm behind the first and the norm before the second:

@@ -2,7 +2,7 @@
 //   dh = dy Wd,  dz = dh u act'(z),  du = dh act(z),  dx = dz Wg + du Wu,  dWg = dz^T x,  dWu = du^T x,  dWd = dy^T h,  biases: column sums.
 // One matrix-product kernel, three epilogues:
 //   kGate   both projections of a tile from one staged x tile, activation and product in registers: h (and, for training, z | u) leave once
-//   kGrad   dh of a tile never leaves: the epilogue reads z | u and writes dz | du and h
+//   kGrad   dh of a tile never leaves: the epilogue reads z | u and writes dz | du
 //   kPlain  C = A B^T (+ bias), or fp32 partial tiles of a cut contraction, summed in order by ff_sum_kernel
 // z | u and dz | du are [rows, 2 hidden]: dx is ONE product over 2 hidden, dWg and dWu are the two halves of ONE product's rows.
 // A product's operands may run along or across the contraction in memory; across, the tile is read transposed (planes.h), so nothing
@@ -10,6 +10,8 @@
 // keeps between its layers: one rounding each), fp32 inputs stay fp32 with three-plane products.
 // Bound: the matrix pipe for many rows, the weights' bytes for few.
 #include "planes.h"
+
+#include <math.h>
 
 namespace eq {
 
@@ -36,7 +38,6 @@ struct FfArgs {
     float* part;                              // [cuts][m][n]
     E* zu;                                    // kGate: written if not null; kGrad: read.  [m, 2 n]
     E* dzu;                                   // kGrad: [m, 2 n]
-    E* h;                                     // kGrad: [m, n]
     int act;
 };
 
@@ -78,13 +79,17 @@ struct FfTile {
     // output r (along): null where there is none, or the last one if clamp (its products are never stored)
     template <class F>
     __device__ __forceinline__ void load(const FfOperand<T>& o, int outer0, int k0, int k_end, F outer_row) {
-        const bool whole = k0 + BK <= k_end && (!kAcross || outer0 + W <= o.len);
+        const bool whole = k0 + BK <= k_end && (!kAcross || o.len % 8 == 0 || outer0 + W <= o.len);      // no chunk is cut
         if (whole) {
 #pragma unroll
             for (int u = 0; u < kPer; ++u) {
                 const int id = threadIdx.x + u * NT, r = id / (W / 8), c = id % (W / 8) * 8;
-                const E* p = kAcross ? o.row(k0 + r) + outer0 + c : outer_row(r, true) + k0 + c;
-                raw[u] = load8<T>(p, 0, 8);
+                if constexpr (kAcross) {
+                    if (outer0 + c < o.len) raw[u] = load8<T>(o.row(k0 + r) + outer0 + c, 0, 8);
+                    else raw[u] = raw_zero<T>();
+                } else {
+                    raw[u] = load8<T>(outer_row(r, true) + k0 + c, 0, 8);
+                }
             }
         } else {
 #pragma unroll
@@ -170,52 +175,72 @@ __global__ __launch_bounds__((FfShapeOf<T, kLarge>::kThreads), 2) void ff_produc
     const int on[2] = {kEpi == kGate ? wn * 32 : wn * 64, kEpi == kGate ? TN + wn * 32 : wn * 64 + 32};
     TA sa;
     TB sb;
-    auto multiply = [&](int buf, auto midway) {
+    // Operands are fetched one step of 16 ahead of their products (two sets of registers): the fence between keeps the compiler from
+    // sinking the reads to their uses, where their latency would be paid at every step.
+    Op8<T> pa[2][MB], pb[2][2];
+    constexpr int KS = BK / 16;
+    auto fetch = [&](int buf, int ks, int set) {
 #pragma unroll
-        for (int ks = 0; ks < BK / 16; ++ks) {
-            Op8<T> pa[MB], pb[2];
+        for (int j = 0; j < 2; ++j) pb[set][j] = TB::operand(tile_b(buf), on[j], ks, lane);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) pb[j] = TB::operand(tile_b(buf), on[j], ks, lane);
-#pragma unroll
-            for (int i = 0; i < MB; ++i) pa[i] = TA::operand(tile_a(buf), om + 32 * i, ks, lane);
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) mma<T>(acc[i][j], pb[j], pa[i]);
-            if (ks == BK / 32 - 1) midway();
-        }
+        for (int i = 0; i < MB; ++i) pa[set][i] = TA::operand(tile_a(buf), om + 32 * i, ks, lane);
+        __builtin_amdgcn_sched_barrier(0);
     };
-    sa.load(g.a, m0, k_begin, k_end, row_a);
-    sb.load(g.b, n0, k_begin, k_end, row_b);
+    auto products = [&](int set) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) mma<T>(acc[i][j], pb[set][j], pa[set][i]);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto load = [&](int k0) {
+        sa.load(g.a, m0, k0, k_end, row_a);
+        sb.load(g.b, n0, k0, k_end, row_b);
+    };
+    auto store = [&](int buf) {
+        sa.store(tile_a(buf));
+        sb.store(tile_b(buf));
+    };
+    load(k_begin);
     if constexpr (NBUF == 2) {
-        sa.store(tile_a(0));
-        sb.store(tile_b(0));
+        // One meeting of the waves per tile, before its last products: the next tile, written halfway, is then readable while those run,
+        // and its memory loads were issued a whole tile earlier.
+        static_assert(KS % 2 == 0, "the next tile starts in the first register set");
+        store(0);
+        if (k_begin + BK < k_end) load(k_begin + BK);
+        __syncthreads();
+        fetch(0, 0, 0);
         int buf = 0;
         for (int k0 = k_begin; k0 < k_end; k0 += BK, buf ^= 1) {
             const bool more = k0 + BK < k_end;
-            if (more) {
-                sa.load(g.a, m0, k0 + BK, k_end, row_a);
-                sb.load(g.b, n0, k0 + BK, k_end, row_b);
-            }
-            __syncthreads();                      // this buffer is written, the other one has been read
-            multiply(buf, [&] {                   // halfway: the loads have arrived, and the waves meet next with nothing left to write
-                if (more) {
-                    sa.store(tile_a(buf ^ 1));
-                    sb.store(tile_b(buf ^ 1));
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + 1 < KS) fetch(buf, ks + 1, (ks + 1) & 1);
+                if (ks == KS / 2 && more) {
+                    store(buf ^ 1);
+                    if (k0 + 2 * BK < k_end) load(k0 + 2 * BK);
                 }
-            });
+                if (ks + 1 == KS && more) {
+                    __syncthreads();
+                    fetch(buf ^ 1, 0, 0);
+                }
+                products(ks & 1);
+            }
         }
     } else {
         for (int k0 = k_begin; k0 < k_end; k0 += BK) {
             __syncthreads();
-            sa.store(tile_a(0));
-            sb.store(tile_b(0));
+            store(0);
             __syncthreads();
-            if (k0 + BK < k_end) {
-                sa.load(g.a, m0, k0 + BK, k_end, row_a);
-                sb.load(g.b, n0, k0 + BK, k_end, row_b);
+            if (k0 + BK < k_end) load(k0 + BK);
+            fetch(0, 0, 0);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + 1 < KS) fetch(0, ks + 1, (ks + 1) & 1);
+                products(ks & 1);
             }
-            multiply(0, [] {});
         }
     }
     __syncthreads();                              // the last tiles have been read
@@ -260,20 +285,17 @@ __global__ __launch_bounds__((FfShapeOf<T, kLarge>::kThreads), 2) void ff_produc
                 }
             } else if constexpr (kEpi == kGrad) {
                 const int64_t at = (int64_t)row * 2 * g.n + col;
-                float h[8];
                 load8f<T>(g.zu + at, left, z);
                 load8f<T>(g.zu + at + g.n, left, u);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float a, d;
                     activate(g.act, z[e], a, d);
-                    h[e] = a * u[e];
                     z[e] = v[e] * u[e] * d;
                     u[e] = v[e] * a;
                 }
                 store8<T>(g.dzu + at, z, left);
                 store8<T>(g.dzu + at + g.n, u, left);
-                store8<T>(g.h + (int64_t)row * g.n + col, h, left);
             } else if (g.cuts > 1) {
                 store8<kF32>(g.part + ((int64_t)cut * g.m + row) * g.n + col, v, left);
             } else {
@@ -295,61 +317,91 @@ __global__ __launch_bounds__(256) void ff_sum_kernel(FfArgs<T> g) {
     const int64_t n = (int64_t)g.m * g.n;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         float v = g.bias ? (float)g.bias[i % g.n] : 0.f;
+#pragma unroll 8
         for (int c = 0; c < g.cuts; ++c) v += g.part[c * n + i];
         store_value<T>(g.c + i, v);
     }
 }
 
-// column sums of [rows, width] (the biases' gradients): runs of rows, then the runs in order
+// The biases' gradients: column sums of dz | du and of dy in one launch, by runs of rows, then the runs in order.  A workgroup takes 64
+// columns of a run, 4 rows at a time.
 template <int T>
-__global__ __launch_bounds__(256) void ff_columns_kernel(const typename Num<T>::type* x, int rows, int width, int run, float* part) {
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6, r0 = blockIdx.y * run, r1 = min(rows, r0 + run);
+struct FfColumns {
+    const typename Num<T>::type* x[2];
+    typename Num<T>::type* out[2];
+    int width[2];                             // 0: not wanted
+    int rows, runs;
+};
+constexpr int kFfRun = 128;                   // rows of a run
+template <int T>
+__global__ __launch_bounds__(256) void ff_columns_kernel(FfColumns<T> a, float* part) {
+    const int first = (a.width[0] + 63) / 64, which = (int)blockIdx.x >= first, block0 = which ? first : 0;
+    const int width = a.width[which], c = ((int)blockIdx.x - block0) * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+    const int r0 = blockIdx.y * kFfRun, r1 = min(a.rows, r0 + kFfRun);
     __shared__ float lds[4][64];
     float v = 0.f;
-    if (c < width)
-        for (int r = r0 + q; r < r1; r += 4) v += (float)x[(int64_t)r * width + c];
+    if (c < width) {
+        const typename Num<T>::type* x = a.x[which] + c;
+#pragma unroll 8
+        for (int r = r0 + q; r < r1; r += 4) v += (float)x[(int64_t)r * width];
+    }
     lds[q][threadIdx.x & 63] = v;
     __syncthreads();
-    if (q == 0 && c < width) part[(int64_t)blockIdx.y * width + c] = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
+    if (q == 0 && c < width)
+        part[(int64_t)blockIdx.y * (a.width[0] + a.width[1]) + (which ? a.width[0] : 0) + c] =
+            (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
 }
 template <int T>
-__global__ __launch_bounds__(256) void ff_columns_sum_kernel(const float* part, int runs, int width, typename Num<T>::type* out) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= width) return;
+__global__ __launch_bounds__(256) void ff_columns_sum_kernel(FfColumns<T> a, const float* part) {
+    const int all = a.width[0] + a.width[1], c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+    __shared__ float lds[4][64];
     float v = 0.f;
-    for (int r = 0; r < runs; ++r) v += part[(int64_t)r * width + c];
-    store_value<T>(out + c, v);
+    if (c < all)
+#pragma unroll 8
+        for (int r = q; r < a.runs; r += 4) v += part[(int64_t)r * all + c];
+    lds[q][threadIdx.x & 63] = v;
+    __syncthreads();
+    if (q || c >= all) return;
+    v = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
+    if (c < a.width[0]) store_value<T>(a.out[0] + c, v);
+    else store_value<T>(a.out[1] + c - a.width[0], v);
 }
 
-struct FfShape { int rows, width, hidden, out; };
-
-// Tile and cuts of a product.  The large tile when it gives at least half the compute units a workgroup; a contraction is cut when the
-// tiles leave compute units idle, into parts of at least 256 (large: 1024) k.
+// Tile and cuts of a product: the cheapest by a model of what was measured (us): a k tile of 64 takes a compute unit 2.2 with one large
+// workgroup, 1.9 with two small ones and 1.2 with one (fp32, k tiles of 32: twice that; odd sizes
+// another half), a workgroup 8 besides; the parts of a cut
+// contraction are written and read at 4 TB/s and cost a launch.  What it decides: large tiles for many outputs, no round of workgroups
+// that is almost empty, cuts for few outputs with a long contraction.
 struct FfPlan { bool large; int tiles_m, tiles_n, cuts, cut_k; };
 static FfPlan ff_plan(int dtype, bool gate, bool can_cut, int m, int n, int k) {
-    FfPlan p;
-    const int columns = gate ? 2 * n : n;
-    p.large = dtype != kF32 && (int64_t)ceil_div(m, 256) * ceil_div(columns, 256) >= 128;
-    const int side = p.large ? 256 : 128, bk = dtype == kF32 ? 32 : 64;
-    p.tiles_m = ceil_div(m, side);
-    p.tiles_n = ceil_div(n, gate ? side / 2 : side);
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, full = p.large ? 256 : 512, least = p.large ? 1024 : 256;
-    int64_t c = 1;
-    if (can_cut && tiles > 0 && tiles <= full / 2) {
-        c = full / tiles;
-        if (c > k / least) c = k / least;
-        if (c < 1) c = 1;
+    FfPlan best = {};
+    double best_cost = 1e30;
+    const int bk = dtype == kF32 ? 32 : 64, k_tiles = k > 0 ? ceil_div(k, bk) : 1;
+    for (int large = 0; large <= (dtype != kF32 ? 1 : 0); ++large) {
+        const int side = large ? 256 : 128, tm = ceil_div(m, side), tn = ceil_div(n, gate ? side / 2 : side);
+        const int64_t tiles = (int64_t)tm * tn;
+        int last = 0;
+        for (int want = 1; want <= (can_cut ? 64 : 1) && want <= k_tiles; ++want) {
+            const int per = ceil_div(k_tiles, want), cuts = ceil_div(k_tiles, per);
+            if (cuts == last) continue;
+            last = cuts;
+            const double blocks = (double)tiles * cuts, tile = (dtype == kF32 ? 2.0 : 1.0) * ((m | n | k) % 8 ? 1.5 : 1.0);
+            double cost;
+            if (large) cost = ceil(blocks / 256) * (2.2 * tile * per + 8);
+            else cost = blocks <= 256 ? 1.2 * tile * per + 8 : ceil(blocks / 512) * (1.9 * tile * per + 8);
+            if (cuts > 1) cost += 5 + (2.0 * cuts + 1) * m * n * 4e-6 / 4;
+            if (cost < best_cost) {
+                best_cost = cost;
+                best = {large != 0, tm, tn, cuts, per * bk};
+            }
+        }
     }
-    p.cut_k = k > 0 ? ceil_div(ceil_div(k, c), bk) * bk : bk;
-    p.cuts = k > 0 ? ceil_div(k, p.cut_k) : 1;
-    return p;
+    return best;
 }
 static int64_t ff_part_size(int dtype, int m, int n, int k) {
     const FfPlan p = ff_plan(dtype, false, true, m, n, k);
     return p.cuts > 1 ? (int64_t)p.cuts * m * n : 0;
 }
-constexpr int kFfRun = 256;                   // rows of a run of a column sum
-
 template <int T, bool kAcrossA, bool kAcrossB, int kEpi>
 static int ff_product(FfArgs<T> g, hipStream_t st, const char* what) {
     const FfPlan p = ff_plan(T, kEpi == kGate, kEpi == kPlain, g.m, g.n, g.k);
@@ -397,18 +449,7 @@ static int ff_forward(const equigspr_gated_feed_forward* d, void* y, void* h, vo
 }
 
 template <int T>
-static int ff_column_sum(const void* x, int rows, int width, float* work, void* out, hipStream_t st) {
-    using E = typename Num<T>::type;
-    const int runs = ceil_div(rows, kFfRun);
-    ff_columns_kernel<T><<<dim3(ceil_div(width, 64), runs), 256, 0, st>>>((const E*)x, rows, width, kFfRun, work);
-    EQ_CHECK_LAUNCH("gated_feed_forward_backward (biases)");
-    ff_columns_sum_kernel<T><<<ceil_div(width, 256), 256, 0, st>>>(work, runs, width, (E*)out);
-    EQ_CHECK_LAUNCH("gated_feed_forward_backward (biases)");
-    return 0;
-}
-
-template <int T>
-static int ff_backward(const equigspr_gated_feed_forward* d, const void* gy, const void* zu, void* h, void* dzu, float* work,
+static int ff_backward(const equigspr_gated_feed_forward* d, const void* gy, const void* zu, const void* h, void* dzu, float* work,
                        const equigspr_gated_feed_forward_grads* o, hipStream_t st) {
     using E = typename Num<T>::type;
     const int r = d->rows, w = d->width, hd = d->hidden, out = d->out;
@@ -418,9 +459,9 @@ static int ff_backward(const equigspr_gated_feed_forward* d, const void* gy, con
     g.a = ff_operand<T>(gy, r, out);
     g.b = ff_operand<T>(d->w_down, out, hd);
     g.m = r; g.n = hd; g.k = out;
-    g.zu = (E*)const_cast<void*>(zu); g.dzu = (E*)dzu; g.h = (E*)h;
+    g.zu = (E*)const_cast<void*>(zu); g.dzu = (E*)dzu;
     if (const int rc = ff_product<T, false, true, kGrad>(g, st, "gated_feed_forward_backward (hidden)")) return rc;
-    g.zu = g.dzu = g.h = nullptr;
+    g.zu = g.dzu = nullptr;
     g.part = work;
     if (o->grad_x) {                          // [dz | du] [Wg ; Wu]
         g.a = ff_operand<T>(dzu, r, 2 * hd);
@@ -445,10 +486,14 @@ static int ff_backward(const equigspr_gated_feed_forward* d, const void* gy, con
         g.c = (E*)o->grad_w_down;
         if (const int rc = ff_product<T, true, true, kPlain>(g, st, "gated_feed_forward_backward (output)")) return rc;
     }
-    if (o->grad_b_gate_up)
-        if (const int rc = ff_column_sum<T>(dzu, r, 2 * hd, work, o->grad_b_gate_up, st)) return rc;
-    if (o->grad_b_down)
-        if (const int rc = ff_column_sum<T>(gy, r, out, work, o->grad_b_down, st)) return rc;
+    if (o->grad_b_gate_up || o->grad_b_down) {
+        FfColumns<T> c = {{(const E*)dzu, (const E*)gy}, {(E*)o->grad_b_gate_up, (E*)o->grad_b_down}, {o->grad_b_gate_up ? 2 * hd : 0, o->grad_b_down ? out : 0},
+                          r, ceil_div(r, kFfRun)};
+        ff_columns_kernel<T><<<dim3(ceil_div(c.width[0], 64) + ceil_div(c.width[1], 64), c.runs), 256, 0, st>>>(c, work);
+        EQ_CHECK_LAUNCH("gated_feed_forward_backward (biases)");
+        ff_columns_sum_kernel<T><<<ceil_div(c.width[0] + c.width[1], 64), 256, 0, st>>>(c, work);
+        EQ_CHECK_LAUNCH("gated_feed_forward_backward (biases' runs)");
+    }
     return 0;
 }
 
@@ -485,13 +530,13 @@ extern "C" int64_t equigspr_gated_feed_forward_backward_work_size(const equigspr
     if (eq::ff_check(d) != 0) return -1;
     int64_t n = eq::ff_part_size(d->dtype, d->rows, d->width, 2 * d->hidden);
     const int64_t up = eq::ff_part_size(d->dtype, 2 * d->hidden, d->width, d->rows), down = eq::ff_part_size(d->dtype, d->out, d->hidden, d->rows);
-    const int64_t widest = 2 * d->hidden > d->out ? 2 * d->hidden : d->out, sums = (int64_t)eq::ceil_div(d->rows, eq::kFfRun) * widest;
+    const int64_t sums = (int64_t)eq::ceil_div(d->rows, eq::kFfRun) * (2 * d->hidden + d->out);
     n = up > n ? up : n;
     n = down > n ? down : n;
     return sums > n ? sums : n;
 }
 
-extern "C" int equigspr_gated_feed_forward_backward(const equigspr_gated_feed_forward* d, const void* grad_y, const void* zu, void* h, void* dzu, float* work,
+extern "C" int equigspr_gated_feed_forward_backward(const equigspr_gated_feed_forward* d, const void* grad_y, const void* zu, const void* h, void* dzu, float* work,
                                                     const equigspr_gated_feed_forward_grads* grads, void* stream) {
     if (const int rc = eq::ff_check(d)) return rc;
     if (d->rows == 0) return 0;

@@ -32,23 +32,23 @@ def _forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, training):
         y, h, zu = new(rows, w_down.shape[0]), new(rows, hidden), new(rows, 2 * hidden) if training else None
         _lib.check(L.equigspr_gated_feed_forward_forward(ctypes.byref(desc), _p(y), _p(h), _p(zu), _p(work), _stream()),
                    "gated_feed_forward_forward")
-    return y, zu
+    return y, zu, h
 
 
 class _FeedForwardFn(torch.autograd.Function):
-    """``equigspr_gated_feed_forward_forward`` / ``_backward``; both projections are kept, everything else is recomputed."""
+    """``equigspr_gated_feed_forward_forward`` / ``_backward``; both projections and the hidden layer are kept."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act):
-        y, zu = _forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, True)
-        ctx.save_for_backward(x, w_gate, w_up, w_down, zu)
+        y, zu, h = _forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, True)
+        ctx.save_for_backward(x, w_gate, w_up, w_down, zu, h)
         ctx.act = act
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        x, w_gate, w_up, w_down, zu = ctx.saved_tensors
+        x, w_gate, w_up, w_down, zu, h = ctx.saved_tensors
         L = _lib.lib()
         need = ctx.needs_input_grad
         rows, width = x.shape
@@ -63,7 +63,7 @@ class _FeedForwardFn(torch.autograd.Function):
             gd = new(out, hidden) if need[3] else None
             gb = new(2 * hidden) if need[4] or need[5] else None
             gbd = new(out) if need[6] else None
-            h, dzu = new(rows, hidden), new(rows, 2 * hidden)
+            dzu = new(rows, 2 * hidden)
             work = torch.empty(max(1, L.equigspr_gated_feed_forward_backward_work_size(ctypes.byref(desc))), dtype=torch.float32, device=x.device)
             ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
             grads = _lib.GatedFeedForwardGrads(ptr(gx), ptr(gw), ptr(gd), ptr(gb), ptr(gbd))
@@ -78,8 +78,8 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
 
     ``x [..., width]``, ``w_gate`` and ``w_up [hidden, width]``, ``w_down [out, hidden]`` (the layout of ``nn.Linear``), biases optional:
     float32, bfloat16 or float16, all alike, on one device (tensors that are not contiguous are copied).  ``activation``: "silu", "gelu"
-    (exact) or "relu".  Products accumulate in fp32; the hidden layer is held in the inputs' dtype between the two products, as the two
-    projections are for the backward: in float16 it must stay within that type's range.  Differentiable once in every tensor; bitwise
+    (exact) or "relu".  Products accumulate in fp32; the hidden layer is held in the inputs' dtype between the two products, as are the
+    two projections and their gradients in the backward: in float16 they must stay within that type's range.  Differentiable once in every tensor; bitwise
     reproducible (no atomics)."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"gated_feed_forward: activation {activation!r}, expected one of {sorted(ACTIVATIONS)}")

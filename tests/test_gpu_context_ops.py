@@ -212,6 +212,13 @@ def test_feed_forward_shapes(dtype, rows, width, hidden, out):
     feed_forward_case(11, dtype, rows, width, hidden, out)
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("rows,width,hidden", [(4100, 512, 1064), (2049, 1030, 1100)])
+def test_feed_forward_large_tiles(dtype, rows, width, hidden):
+    """Enough outputs for the large tile in every product, with tiles cut at every edge, and contractions cut into parts."""
+    feed_forward_case(14, dtype, rows, width, hidden)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("activation", ["silu", "gelu", "relu"])
 @pytest.mark.parametrize("biased", [True, False])
