@@ -129,16 +129,39 @@ typedef pf32x4 pf32x4_u __attribute__((aligned(4)));
 typedef s16x8 s16x8_u __attribute__((aligned(2)));
 typedef s16x4 s16x4_u __attribute__((aligned(2)));
 
-// eight values at row + col of a row of `width` values; those at or behind the end are zero
+// eight values at row + col of a row of `width` values; those at or behind the end are zero.  The row's last eight values are loaded for a
+// chunk that crosses the end, and moved down (one load for every lane; value by value, the edge tiles of odd sizes took three times as
+// long as the others).
 template <int T>
 __device__ __forceinline__ Raw8<T> load8(const typename Num<T>::type* row, int col, int width) {
     Raw8<T> r;
-    if (col + 8 <= width) {
+    if (width >= 8) {
+        const int start = min(col, width - 8), move = col - start;
         if constexpr (T == kF32) {
-            r.v[0] = *reinterpret_cast<const pf32x4_u*>(row + col);
-            r.v[1] = *reinterpret_cast<const pf32x4_u*>(row + col + 4);
+            r.v[0] = *reinterpret_cast<const pf32x4_u*>(row + start);
+            r.v[1] = *reinterpret_cast<const pf32x4_u*>(row + start + 4);
+            if (move > 0) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = r.v[i >> 2][i & 3];
+#pragma unroll
+                for (int k = 0; k < 3; ++k)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = move & (1 << k) ? (i + (1 << k) < 8 ? x[i + (1 << k)] : 0.f) : x[i];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r.v[i >> 2][i & 3] = move < 8 ? x[i] : 0.f;
+            }
         } else {
-            r.v = *reinterpret_cast<const s16x8_u*>(row + col);
+            r.v = *reinterpret_cast<const s16x8_u*>(row + start);
+            if (move > 0) {
+                typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+                const u64x2 w = __builtin_bit_cast(u64x2, r.v);
+                const int bits = 16 * (move & 3);
+                u64x2 o = {bits ? (w[0] >> bits) | (w[1] << (64 - bits)) : w[0], w[1] >> bits};
+                if (move >= 4) o = (u64x2){o[1], 0};
+                if (move >= 8) o = (u64x2){0, 0};
+                r.v = __builtin_bit_cast(s16x8, o);
+            }
         }
     } else {
         r = raw_zero<T>();

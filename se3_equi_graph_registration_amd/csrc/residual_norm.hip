@@ -39,274 +39,270 @@ struct NormArgs {
     int want;                                 // bit i: partial i is wanted; bit 5: the gate's gradient
 };
 
-// L threads own a row, PER chunks of eight columns each; NT threads of a workgroup own NT / L rows at a time
+// L threads own a row, eight consecutive columns each; NT threads of a workgroup own NT / L rows at a time.  Sums over a row: one meeting
+// of the workgroup each (two buffers in turn: whoever writes one again has met everybody since they read it).
 template <int L, int NT>
-__device__ __forceinline__ float row_sum(float v, float* lds) {
-    if constexpr (L <= 64) {
+struct RowSums {
+    float* lds;                               // [2][2][NT / 64]
+    int turn;
+    __device__ __forceinline__ void sum(float& a, float& b) {
 #pragma unroll
-        for (int o = L / 2; o; o >>= 1) v += __shfl_xor(v, o);
-        return v;
-    } else {
+        for (int o = (L < 64 ? L : 64) / 2; o; o >>= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
+        if constexpr (L > 64) {
+            float* s = lds + turn * 2 * (NT / 64);
+            turn ^= 1;
+            if ((threadIdx.x & 63) == 0) { s[threadIdx.x >> 6] = a; s[NT / 64 + (threadIdx.x >> 6)] = b; }
+            __syncthreads();
+            a = b = 0.f;
 #pragma unroll
-        for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-        __syncthreads();                      // the previous sum has been read
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-        __syncthreads();
-        float t = 0.f;
-#pragma unroll
-        for (int i = 0; i < NT / 64; ++i) t += lds[i];
-        return t;
-    }
-}
-
-template <int T, int L, int PER>
-struct Row {
-    float v[PER * 8];
-    __device__ __forceinline__ void load(const typename Num<T>::type* row, int width, int t) {
-#pragma unroll
-        for (int c = 0; c < PER; ++c) {
-            const int col = (c * L + t) * 8;
-            const Raw8<T> r = row && col < width ? load8<T>(row, col, width) : raw_zero<T>();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[c * 8 + i] = raw_float<T>(r, i);
+            for (int i = 0; i < NT / 64; ++i) { a += s[i]; b += s[NT / 64 + i]; }
         }
     }
-    __device__ __forceinline__ void store(typename Num<T>::type* row, int width, int t) const {
-#pragma unroll
-        for (int c = 0; c < PER; ++c) {
-            const int col = (c * L + t) * 8;
-            if (col < width) {
-                float a[4], b[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) { a[i] = v[c * 8 + i]; b[i] = v[c * 8 + 4 + i]; }
-                store4<T>(row + col, a, width - col);
-                if (col + 4 < width) store4<T>(row + col + 4, b, width - col - 4);
-            }
-        }
+    __device__ __forceinline__ float sum(float a) {
+        float b = 0.f;
+        sum(a, b);
+        return a;
     }
 };
 
-template <int L, int PER>
-__device__ __forceinline__ void load_columns(float (&w)[PER * 8], const float* p, int width, int t, float otherwise) {
+template <int T>
+__device__ __forceinline__ Raw8<T> load_row(const typename Num<T>::type* row, int width, int col) {
+    return row && col < width ? load8<T>(row, col, width) : raw_zero<T>();
+}
+template <int T>
+__device__ __forceinline__ void row_values(const Raw8<T>& r, float (&v)[8]) {
 #pragma unroll
-    for (int c = 0; c < PER; ++c) {
-        const int col = (c * L + t) * 8;
+    for (int i = 0; i < 8; ++i) v[i] = raw_float<T>(r, i);
+}
+__device__ __forceinline__ void load_columns(const float* p, int width, int col, float otherwise, float (&w)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[c * 8 + i] = otherwise;
-        if (p && col < width) {
-            const Raw8<kF32> r = load8<kF32>(p, col, width);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[c * 8 + i] = raw_float<kF32>(r, i);
-        }
-    }
+    for (int i = 0; i < 8; ++i) w[i] = otherwise;
+    if (p && col < width) row_values<kF32>(load8<kF32>(p, col, width), w);
 }
 
 // v -> its unit row in place (columns behind the width become zero); returns 1 / spread
-template <int L, int PER, int NT>
-__device__ __forceinline__ float unit_row(float (&v)[PER * 8], int rms, float eps, int width, int t, float* lds) {
+template <bool kRms, class S>
+__device__ __forceinline__ float unit_row(float (&v)[8], float eps, int width, int col, S& sums) {
     const float inv = 1.f / (float)width;
-    if (!rms) {
+    if constexpr (!kRms) {
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < PER * 8; ++i) sum += v[i];
-        const float mean = row_sum<L, NT>(sum, lds) * inv;
+        for (int i = 0; i < 8; ++i) sum += v[i];
+        const float mean = sums.sum(sum) * inv;
 #pragma unroll
-        for (int c = 0; c < PER; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[c * 8 + i] = (c * L + t) * 8 + i < width ? v[c * 8 + i] - mean : 0.f;
+        for (int i = 0; i < 8; ++i) v[i] = col + i < width ? v[i] - mean : 0.f;
     }
     float sq = 0.f;
 #pragma unroll
-    for (int i = 0; i < PER * 8; ++i) sq = fmaf(v[i], v[i], sq);
-    const float r = 1.f / sqrtf(row_sum<L, NT>(sq, lds) * inv + eps);
+    for (int i = 0; i < 8; ++i) sq = fmaf(v[i], v[i], sq);
+    const float r = 1.f / sqrtf(sums.sum(sq) * inv + eps);
 #pragma unroll
-    for (int i = 0; i < PER * 8; ++i) v[i] *= r;
+    for (int i = 0; i < 8; ++i) v[i] *= r;
     return r;
 }
 
-template <int T, int L, int PER, int NT>
-__global__ __launch_bounds__(NT) void norm_fwd_kernel(NormArgs<T> a) {
-    const NormShape& s = a.s;
-    __shared__ float lds[NT / 64];
-    const int t = threadIdx.x % L;
-    const int64_t step = (int64_t)gridDim.x * (NT / L);
-    for (int64_t r0 = (int64_t)blockIdx.x * (NT / L); r0 < s.rows; r0 += step) {
-        const int64_t row = r0 + threadIdx.x / L;
-        const bool ok = row < s.rows;
-        const int64_t at = row * s.width;
-        Row<T, L, PER> x, f;
-        x.load(ok ? a.x + at : nullptr, s.width, t);
-        f.load(ok && a.f ? a.f + at : nullptr, s.width, t);
-        float w[PER * 8];
-        if (s.post) {
-            unit_row<L, PER, NT>(f.v, s.rms, s.eps, s.width, t, lds);
-            load_columns<L, PER>(w, s.post_w, s.width, t, 1.f);
-#pragma unroll
-            for (int i = 0; i < PER * 8; ++i) f.v[i] *= w[i];
-            if (s.post_b) {
-                load_columns<L, PER>(w, s.post_b, s.width, t, 0.f);
-#pragma unroll
-                for (int i = 0; i < PER * 8; ++i) f.v[i] += w[i];
-            }
-        }
-        load_columns<L, PER>(w, s.scale, s.width, t, s.factor);
-        if (a.gate) {
-            Row<T, L, PER> g;
-            g.load(ok ? a.gate + row / s.gate_rows * s.width : nullptr, s.width, t);
-#pragma unroll
-            for (int i = 0; i < PER * 8; ++i) w[i] *= g.v[i];
-        }
-#pragma unroll
-        for (int i = 0; i < PER * 8; ++i) x.v[i] = fmaf(w[i], f.v[i], x.v[i]);
-        if (ok && a.y) x.store(a.y + at, s.width, t);
-        if (s.pre) {
-            unit_row<L, PER, NT>(x.v, s.rms, s.eps, s.width, t, lds);
-            load_columns<L, PER>(w, s.pre_w, s.width, t, 1.f);
-#pragma unroll
-            for (int i = 0; i < PER * 8; ++i) x.v[i] *= w[i];
-            if (s.pre_b) {
-                load_columns<L, PER>(w, s.pre_b, s.width, t, 0.f);
-#pragma unroll
-                for (int i = 0; i < PER * 8; ++i) x.v[i] += w[i];
-            }
-            if (ok) x.store(a.u + at, s.width, t);
-        }
-    }
-}
-
 // g <- gradient of the rows whose unit rows are n: (g - [layer: mean g] - n mean(g n)) r
-template <int L, int PER, int NT>
-__device__ __forceinline__ void unit_row_grad(float (&g)[PER * 8], const float (&n)[PER * 8], float r, int rms, int width, int t, float* lds) {
+template <bool kRms, class S>
+__device__ __forceinline__ void unit_row_grad(float (&g)[8], const float (&n)[8], float r, int width, int col, S& sums) {
     const float inv = 1.f / (float)width;
     float sg = 0.f, sn = 0.f;
 #pragma unroll
-    for (int i = 0; i < PER * 8; ++i) { sg += g[i]; sn = fmaf(g[i], n[i], sn); }
-    sn = row_sum<L, NT>(sn, lds) * inv;
-    sg = rms ? 0.f : row_sum<L, NT>(sg, lds) * inv;
+    for (int i = 0; i < 8; ++i) {
+        if (!kRms) sg += g[i];
+        sn = fmaf(g[i], n[i], sn);
+    }
+    sums.sum(sn, sg);
+    sn *= inv;
+    sg *= inv;
 #pragma unroll
-    for (int c = 0; c < PER; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int k = c * 8 + i;
-            g[k] = (c * L + t) * 8 + i < width ? (g[k] - sg - n[k] * sn) * r : 0.f;
-        }
+    for (int i = 0; i < 8; ++i) g[i] = col + i < width ? (g[i] - (kRms ? 0.f : sg) - n[i] * sn) * r : 0.f;
 }
 
-// sums acc over the row groups of the workgroup and writes (or rounds) one row of width values
-template <int L, int PER, int NT, class F>
-__device__ __forceinline__ void group_columns(const float (&acc)[PER * 8], float* lds, int width, F put) {
-    const int t = threadIdx.x % L, grp = threadIdx.x / L;
-    if constexpr (NT == L) {
+// The parameters of a thread's columns stay in registers while it walks its rows, and the next row is loaded under this row's arithmetic;
+// the widest rows (1024 threads, 128 registers each) have no room for either.
+template <int T, int L, int NT, bool kRms>
+__global__ __launch_bounds__(NT) void norm_fwd_kernel(NormArgs<T> a) {
+    constexpr bool kAhead = NT < 1024;
+    const NormShape& s = a.s;
+    __shared__ float lds[4 * (NT / 64)];
+    RowSums<L, NT> sums = {lds, 0};
+    const int col = threadIdx.x % L * 8;
+    const int64_t step = (int64_t)gridDim.x * (NT / L), first = (int64_t)blockIdx.x * (NT / L);
+    float post_w[8], post_b[8], pre_w[8], pre_b[8], scale[8];
+    auto params = [&] {
+        load_columns(s.post_w, s.width, col, 1.f, post_w);
+        load_columns(s.post_b, s.width, col, 0.f, post_b);
+        load_columns(s.pre_w, s.width, col, 1.f, pre_w);
+        load_columns(s.pre_b, s.width, col, 0.f, pre_b);
+        load_columns(s.scale, s.width, col, s.factor, scale);
+    };
+    Raw8<T> nx, nf;
+    auto load = [&](int64_t r0) {
+        const int64_t row = r0 + threadIdx.x / L;
+        const bool ok = row < s.rows;
+        nx = load_row<T>(ok ? a.x + row * s.width : nullptr, s.width, col);
+        nf = load_row<T>(ok && a.f ? a.f + row * s.width : nullptr, s.width, col);
+    };
+    if (kAhead) {
+        params();
+        load(first);
+    }
+    for (int64_t r0 = first; r0 < s.rows; r0 += step) {
+        const int64_t row = r0 + threadIdx.x / L, at = row * s.width + col;
+        const bool ok = row < s.rows && col < s.width;
+        float x[8], f[8], w[8];
+        if (!kAhead) load(r0);
+        row_values<T>(nx, x);
+        row_values<T>(nf, f);
+        if (kAhead && r0 + step < s.rows) load(r0 + step);
+        if (!kAhead) params();
+        if (s.post) {
+            unit_row<kRms>(f, s.eps, s.width, col, sums);
 #pragma unroll
-        for (int c = 0; c < PER; ++c)
+            for (int i = 0; i < 8; ++i) f[i] = fmaf(f[i], post_w[i], post_b[i]);
+        }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if ((c * L + t) * 8 + i < width) put((c * L + t) * 8 + i, acc[c * 8 + i]);
-    } else {
-        constexpr int kCols = L * PER * 8;
-        __syncthreads();
+        for (int i = 0; i < 8; ++i) w[i] = scale[i];
+        if (a.gate) {
+            float g[8];
+            row_values<T>(load_row<T>(row < s.rows ? a.gate + row / s.gate_rows * s.width : nullptr, s.width, col), g);
 #pragma unroll
-        for (int c = 0; c < PER; ++c)
+            for (int i = 0; i < 8; ++i) w[i] *= g[i];
+        }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) lds[grp * kCols + (c * L + t) * 8 + i] = acc[c * 8 + i];
-        __syncthreads();
-        for (int col = threadIdx.x; col < width; col += NT) {
-            float v = 0.f;
-            for (int q = 0; q < NT / L; ++q) v += lds[q * kCols + col];
-            put(col, v);
+        for (int i = 0; i < 8; ++i) x[i] = fmaf(w[i], f[i], x[i]);
+        if (ok && a.y) store8<T>(a.y + at, x, s.width - col);
+        if (s.pre) {
+            unit_row<kRms>(x, s.eps, s.width, col, sums);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], pre_w[i], pre_b[i]);
+            if (ok) store8<T>(a.u + at, x, s.width - col);
         }
     }
 }
 
-template <int T, int L, int PER, int NT>
-__global__ __launch_bounds__(NT) void norm_bwd_kernel(NormArgs<T> a) {
-    constexpr int V = PER * 8, G = NT / L;
-    const NormShape& s = a.s;
-    __shared__ float lds[NT / 64];
-    __shared__ float cols[G > 1 ? G * L * V : 1];
-    const int t = threadIdx.x % L;
-    float s_prew[V], s_preb[V], s_postw[V], s_postb[V], s_scale[V];
+// sums acc over the row groups of the workgroup and hands out one row of width values
+template <int L, int NT, class F>
+__device__ __forceinline__ void group_columns(const float (&acc)[8], float* lds, int width, F put) {
+    const int col = threadIdx.x % L * 8;
+    if constexpr (NT == L) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) s_prew[i] = s_preb[i] = s_postw[i] = s_postb[i] = s_scale[i] = 0.f;
+        for (int i = 0; i < 8; ++i)
+            if (col + i < width) put(col + i, acc[i]);
+    } else {
+        constexpr int kCols = L * 8;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) lds[threadIdx.x / L * kCols + col + i] = acc[i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < width; c += NT) {
+            float v = 0.f;
+            for (int q = 0; q < NT / L; ++q) v += lds[q * kCols + c];
+            put(c, v);
+        }
+    }
+}
+
+template <int T, int L, int NT, bool kRms>
+__global__ __launch_bounds__(NT) void norm_bwd_kernel(NormArgs<T> a) {
+    constexpr int G = NT / L;
+    constexpr bool kAhead = NT < 1024;
+    const NormShape& s = a.s;
+    __shared__ float lds[4 * (NT / 64)];
+    __shared__ float cols[G > 1 ? G * L * 8 : 1];
+    RowSums<L, NT> sums = {lds, 0};
+    const int col = threadIdx.x % L * 8;
+    float post_w[8], post_b[8], pre_w[8], scale[8], gate[8];
+    float s_prew[8], s_preb[8], s_postw[8], s_postb[8], s_scale[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { s_prew[i] = s_preb[i] = s_postw[i] = s_postb[i] = s_scale[i] = 0.f; gate[i] = 1.f; }
+    auto params = [&] {
+        load_columns(s.post_w, s.width, col, 1.f, post_w);
+        load_columns(s.post_b, s.width, col, 0.f, post_b);
+        load_columns(s.pre_w, s.width, col, 1.f, pre_w);
+        load_columns(s.scale, s.width, col, s.factor, scale);
+    };
+    if (kAhead) params();
     for (int64_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
         const int64_t gate_row = unit / a.cuts, first = gate_row * s.gate_rows + (unit - gate_row * a.cuts) * a.unit_rows;
         const int64_t group_end = (gate_row + 1) * s.gate_rows, end0 = first + a.unit_rows, end = end0 < group_end ? end0 : group_end;
-        float s_gate[V];
+        float s_z[8];                         // sum of grad_y_total * z: the gate's gradient up to the scale, the scale's up to the gate
 #pragma unroll
-        for (int i = 0; i < V; ++i) s_gate[i] = 0.f;
-        for (int64_t r0 = first; r0 < end; r0 += G) {
+        for (int i = 0; i < 8; ++i) s_z[i] = 0.f;
+        if (a.gate) row_values<T>(load_row<T>(a.gate + gate_row * s.width, s.width, col), gate);
+        Raw8<T> nx, nf, ngy, ngu;
+        auto load = [&](int64_t r0) {
             const int64_t row = r0 + threadIdx.x / L, at = row * s.width;
-            const bool ok = row < end && row < s.rows;
-            Row<T, L, PER> x, f, gu, gy;
-            f.load(ok && a.f ? a.f + at : nullptr, s.width, t);
-            x.load(ok ? a.x + at : nullptr, s.width, t);
-            gu.load(ok && a.gu ? a.gu + at : nullptr, s.width, t);
-            gy.load(ok && a.gy ? a.gy + at : nullptr, s.width, t);
-            float w[V], z[V], fr = 1.f;
+            const bool ok = row < end;
+            nf = load_row<T>(ok && a.f ? a.f + at : nullptr, s.width, col);
+            nx = load_row<T>(ok ? a.x + at : nullptr, s.width, col);
+            ngu = load_row<T>(ok && a.gu ? a.gu + at : nullptr, s.width, col);
+            ngy = load_row<T>(ok && a.gy ? a.gy + at : nullptr, s.width, col);
+        };
+        if (kAhead) load(first);
+        for (int64_t r0 = first; r0 < end; r0 += G) {
+            const int64_t row = r0 + threadIdx.x / L, at = row * s.width + col;
+            const bool ok = row < end && col < s.width;
+            float x[8], f[8], gy[8], gu[8], z[8], fr = 1.f;
+            if (!kAhead) load(r0);
+            row_values<T>(nf, f);
+            row_values<T>(nx, x);
+            row_values<T>(ngu, gu);
+            row_values<T>(ngy, gy);
+            if (kAhead && r0 + G < end) load(r0 + G);
+            if (!kAhead) params();
             if (s.post) {
-                fr = unit_row<L, PER, NT>(f.v, s.rms, s.eps, s.width, t, lds);
-                load_columns<L, PER>(w, s.post_w, s.width, t, 1.f);
+                fr = unit_row<kRms>(f, s.eps, s.width, col, sums);
 #pragma unroll
-                for (int i = 0; i < V; ++i) z[i] = f.v[i] * w[i];
-                if (s.post_b) {
-                    load_columns<L, PER>(w, s.post_b, s.width, t, 0.f);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) z[i] += w[i];
-                }
+                for (int i = 0; i < 8; ++i) z[i] = fmaf(f[i], post_w[i], post_b[i]);
             } else {
 #pragma unroll
-                for (int i = 0; i < V; ++i) z[i] = f.v[i];
+                for (int i = 0; i < 8; ++i) z[i] = f[i];
             }
-            float sc[V];
-            Row<T, L, PER> gt;
-            load_columns<L, PER>(sc, s.scale, s.width, t, s.factor);
-            if (a.gate) gt.load(ok ? a.gate + gate_row * s.width : nullptr, s.width, t);
-            else
-#pragma unroll
-                for (int i = 0; i < V; ++i) gt.v[i] = 1.f;
             if (s.pre) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) x.v[i] = fmaf(sc[i] * gt.v[i], z[i], x.v[i]);
-                const float yr = unit_row<L, PER, NT>(x.v, s.rms, s.eps, s.width, t, lds);
-                load_columns<L, PER>(w, s.pre_w, s.width, t, 1.f);
+                for (int i = 0; i < 8; ++i) x[i] = fmaf(scale[i] * gate[i], z[i], x[i]);
+                const float yr = unit_row<kRms>(x, s.eps, s.width, col, sums);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    s_prew[i] = fmaf(gu.v[i], x.v[i], s_prew[i]);
-                    s_preb[i] += gu.v[i];
-                    gu.v[i] *= w[i];
+                for (int i = 0; i < 8; ++i) {
+                    s_prew[i] = fmaf(gu[i], x[i], s_prew[i]);
+                    if (!kRms || s.pre_b) s_preb[i] += gu[i];
+                    gu[i] *= pre_w[i];
                 }
-                unit_row_grad<L, PER, NT>(gu.v, x.v, yr, s.rms, s.width, t, lds);
+                unit_row_grad<kRms>(gu, x, yr, s.width, col, sums);
 #pragma unroll
-                for (int i = 0; i < V; ++i) gy.v[i] += gu.v[i];
+                for (int i = 0; i < 8; ++i) gy[i] += gu[i];
             }
-            if (ok && a.gx) gy.store(a.gx + at, s.width, t);
+            if (ok && a.gx) store8<T>(a.gx + at, gy, s.width - col);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float gz = gy.v[i] * z[i];
-                s_gate[i] = fmaf(gz, sc[i], s_gate[i]);
-                s_scale[i] = fmaf(gz, gt.v[i], s_scale[i]);
-                gy.v[i] *= sc[i] * gt.v[i];
+            for (int i = 0; i < 8; ++i) {
+                s_z[i] = fmaf(gy[i], z[i], s_z[i]);
+                gy[i] *= scale[i] * gate[i];
             }
             if (s.post) {
-                load_columns<L, PER>(w, s.post_w, s.width, t, 1.f);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    s_postw[i] = fmaf(gy.v[i], f.v[i], s_postw[i]);
-                    s_postb[i] += gy.v[i];
-                    gy.v[i] *= w[i];
+                for (int i = 0; i < 8; ++i) {
+                    s_postw[i] = fmaf(gy[i], f[i], s_postw[i]);
+                    if (!kRms || s.post_b) s_postb[i] += gy[i];
+                    gy[i] *= post_w[i];
                 }
-                if (a.gf) unit_row_grad<L, PER, NT>(gy.v, f.v, fr, s.rms, s.width, t, lds);
+                if (a.gf) unit_row_grad<kRms>(gy, f, fr, s.width, col, sums);
             }
-            if (ok && a.gf) gy.store(a.gf + at, s.width, t);
+            if (ok && a.gf) store8<T>(a.gf + at, gy, s.width - col);
         }
+        if (!kAhead) params();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s_scale[i] = fmaf(s_z[i], gate[i], s_scale[i]);
         if (a.want & 32) {
-            if (a.cuts == 1) group_columns<L, PER, NT>(s_gate, cols, s.width, [&](int c, float v) { store_value<T>(a.ggate + gate_row * s.width + c, v); });
-            else group_columns<L, PER, NT>(s_gate, cols, s.width, [&](int c, float v) { a.gate_part[unit * s.width + c] = v; });
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s_z[i] *= scale[i];
+            if (a.cuts == 1) group_columns<L, NT>(s_z, cols, s.width, [&](int c, float v) { store_value<T>(a.ggate + gate_row * s.width + c, v); });
+            else group_columns<L, NT>(s_z, cols, s.width, [&](int c, float v) { a.gate_part[unit * s.width + c] = v; });
         }
     }
-    auto put = [&](int k, const float (&acc)[V]) {
+    auto put = [&](int k, const float (&acc)[8]) {
         if (a.want >> k & 1)
-            group_columns<L, PER, NT>(acc, cols, s.width, [&](int c, float v) { a.part[((int64_t)k * gridDim.x + blockIdx.x) * s.width + c] = v; });
+            group_columns<L, NT>(acc, cols, s.width, [&](int c, float v) { a.part[((int64_t)k * gridDim.x + blockIdx.x) * s.width + c] = v; });
     };
     put(0, s_prew);
     put(1, s_preb);
@@ -317,40 +313,40 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(NormArgs<T> a) {
 
 struct NormColumns { float* out[5]; };
 
-// out[k] = sum over the workgroups' partial rows, in order: 64 columns x 4 runs of rows per workgroup
-__global__ __launch_bounds__(256) void norm_columns_kernel(const float* part, int parts, int width, NormColumns o) {
-    __shared__ float lds[4][64];
-    const int k = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
-    if (!o.out[k]) return;
+// The parameters' gradients (blockIdx.y 0..4: sums of the workgroups' partial rows) and the gate's (from 5 on: a gate row from its cuts),
+// in order: 16 columns x 16 runs of rows per workgroup, the runs joined in LDS.
+template <int T>
+__global__ __launch_bounds__(256) void norm_columns_kernel(const float* part, int parts, const float* gate_part, int cuts, int width, NormColumns o,
+                                                           typename Num<T>::type* ggate) {
+    __shared__ float lds[16][17];
+    const int k = blockIdx.y, c = blockIdx.x * 16 + (threadIdx.x & 15), q = threadIdx.x >> 4;
+    if (k < 5 && !o.out[k]) return;
+    const int n = k < 5 ? parts : cuts;
+    const float* p = (k < 5 ? part + (int64_t)k * parts * width : gate_part + (int64_t)(k - 5) * cuts * width) + c;
     float v = 0.f;
     if (c < width)
-        for (int p = q; p < parts; p += 4) v += part[((int64_t)k * parts + p) * width + c];
-    lds[q][threadIdx.x & 63] = v;
+#pragma unroll 8
+        for (int i = q; i < n; i += 16) v += p[(int64_t)i * width];
+    lds[q][threadIdx.x & 15] = v;
     __syncthreads();
-    if (q == 0 && c < width) o.out[k][c] = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
-}
-
-// a gate row's gradient from its cuts, in order
-template <int T>
-__global__ __launch_bounds__(256) void norm_gate_kernel(const float* part, int cuts, int width, typename Num<T>::type* out) {
-    const int64_t g = blockIdx.y;
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= width) return;
-    float v = 0.f;
-    for (int p = 0; p < cuts; ++p) v += part[(g * cuts + p) * width + c];
-    store_value<T>(out + g * width + c, v);
+    if (threadIdx.x >= 16 || c >= width) return;
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v += lds[i][threadIdx.x];
+    if (k < 5) o.out[k][c] = v;
+    else store_value<T>(ggate + (int64_t)(k - 5) * width + c, v);
 }
 
 // threads of a row and of a workgroup by the width: the row fits the registers, narrow rows share a wave
 static int norm_group_rows(int width) { return width <= 64 ? 32 : width <= 512 ? 4 : 1; }
 
 struct NormPlan { int64_t units; int unit_rows, cuts, blocks; };
-// Backward: up to 1024 workgroups.  With a gate, a unit is a run of rows of one gate row (a gate row with many rows is cut); without,
-// a run of rows.
+// Backward: up to 768 workgroups (three per compute unit).  With a gate, a unit is a run of rows of one gate row (a gate row with many
+// rows is cut); without, a run of rows.
 static NormPlan norm_plan(const NormShape& s, bool gated) {
     NormPlan p;
     const int g = norm_group_rows(s.width);
-    const int64_t groups = s.rows / s.gate_rows, most = 1024;
+    const int64_t groups = s.rows / s.gate_rows, most = 768;
     int64_t cuts = groups >= most ? 1 : most / groups;
     const int64_t room = (s.gate_rows + g - 1) / g;
     if (cuts > room) cuts = room;
@@ -364,16 +360,18 @@ static NormPlan norm_plan(const NormShape& s, bool gated) {
 template <int T>
 static int norm_run(const NormArgs<T>& a, bool backward, int blocks, hipStream_t st) {
     const int w = a.s.width;
-#define EQ_NORM(L, PER, NT)                                                            \
-    do {                                                                               \
-        if (backward) norm_bwd_kernel<T, L, PER, NT><<<blocks, NT, 0, st>>>(a);        \
-        else norm_fwd_kernel<T, L, PER, NT><<<blocks, NT, 0, st>>>(a);                 \
+#define EQ_NORM(L, NT)                                                                              \
+    do {                                                                                            \
+        if (backward && a.s.rms) norm_bwd_kernel<T, L, NT, true><<<blocks, NT, 0, st>>>(a);         \
+        else if (backward) norm_bwd_kernel<T, L, NT, false><<<blocks, NT, 0, st>>>(a);              \
+        else if (a.s.rms) norm_fwd_kernel<T, L, NT, true><<<blocks, NT, 0, st>>>(a);                \
+        else norm_fwd_kernel<T, L, NT, false><<<blocks, NT, 0, st>>>(a);                            \
     } while (0)
-    if (w <= 64) EQ_NORM(8, 1, 256);
-    else if (w <= 512) EQ_NORM(64, 1, 256);
-    else if (w <= 2048) EQ_NORM(256, 1, 256);
-    else if (w <= 4096) EQ_NORM(512, 1, 512);
-    else EQ_NORM(1024, 1, 1024);
+    if (w <= 64) EQ_NORM(8, 256);
+    else if (w <= 512) EQ_NORM(64, 256);
+    else if (w <= 2048) EQ_NORM(256, 256);
+    else if (w <= 4096) EQ_NORM(512, 512);
+    else EQ_NORM(1024, 1024);
 #undef EQ_NORM
     EQ_CHECK_LAUNCH(backward ? "residual_norm_backward" : "residual_norm_forward");
     return 0;
@@ -406,7 +404,7 @@ static int norm_forward(const equigspr_residual_norm* d, const NormShape& s, voi
     a.x = (const E*)d->x; a.f = (const E*)d->f; a.gate = (const E*)d->gate;
     a.y = (E*)y; a.u = (E*)u;
     const int64_t groups = (s.rows + norm_group_rows(s.width) - 1) / norm_group_rows(s.width);
-    return norm_run<T>(a, false, (int)(groups < 8192 ? groups : 8192), st);
+    return norm_run<T>(a, false, (int)(groups < 2048 ? groups : 2048), st);
 }
 
 template <int T>
@@ -428,13 +426,11 @@ static int norm_backward(const equigspr_residual_norm* d, const NormShape& s, co
     a.part = work;
     a.gate_part = work + (int64_t)5 * p.blocks * s.width;
     if (const int rc = norm_run<T>(a, true, p.blocks, st)) return rc;
-    if (columns) {
-        norm_columns_kernel<<<dim3(ceil_div(s.width, 64), 5), 256, 0, st>>>(a.part, p.blocks, s.width, c);
+    const bool gate_cut = a.ggate && p.cuts > 1;
+    if (columns || gate_cut) {
+        norm_columns_kernel<T><<<dim3(ceil_div(s.width, 16), 5 + (gate_cut ? (unsigned)(s.rows / s.gate_rows) : 0)), 256, 0, st>>>(
+            a.part, p.blocks, a.gate_part, p.cuts, s.width, c, a.ggate);
         EQ_CHECK_LAUNCH("residual_norm_backward (columns)");
-    }
-    if (a.ggate && p.cuts > 1) {
-        norm_gate_kernel<T><<<dim3(ceil_div(s.width, 256), (unsigned)(s.rows / s.gate_rows)), 256, 0, st>>>(a.gate_part, p.cuts, s.width, a.ggate);
-        EQ_CHECK_LAUNCH("residual_norm_backward (gate)");
     }
     return 0;
 }

@@ -207,7 +207,8 @@ def feed_forward_case(seed, dtype, rows, width, hidden, out=None, activation="si
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("rows,width,hidden,out", [(1, 1, 1, 1), (1, 32, 128, 32), (5, 33, 70, 33), (64, 32, 128, 48), (130, 129, 65, 20), (300, 64, 200, 64),
-                                                   (1000, 40, 72, 40), (17, 512, 300, 256), (16, 640, 1280, 640), (33, 100, 1030, 7)])
+                                                   (1000, 40, 72, 40), (17, 512, 300, 256), (16, 640, 1280, 640), (33, 100, 1030, 7),
+                                                   (2, 2100, 300, 33), (32, 130, 1500, 130), (9, 8, 17, 3)])
 def test_feed_forward_shapes(dtype, rows, width, hidden, out):
     feed_forward_case(11, dtype, rows, width, hidden, out)
 
