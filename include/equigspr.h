@@ -526,14 +526,14 @@ typedef struct equigspr_attention {
     int64_t mask_stride;
 } equigspr_attention;
 
-/* out [batch, nq, heads, dim] contiguous; lse (optional, for the backward) [batch, kv_heads, nq * heads / kv_heads] floats;
- * work: equigspr_attention_work_size floats (0: may be null) */
+/* out [batch, nq, heads, dim] contiguous; for the backward (optional): lse [batch, kv_heads, nq * heads / kv_heads] floats, and, 16-bit
+ * types, out_low, shaped like out: what out's rounding dropped; work: equigspr_attention_work_size floats (0: may be null) */
 int64_t equigspr_attention_work_size(const equigspr_attention* desc);
-int equigspr_attention_forward(const equigspr_attention* desc, void* out, float* lse, float* work, void* stream);
-/* out, lse: as the forward wrote them; grad_q / grad_k / grad_v: contiguous, written (not accumulated), each may be null.
+int equigspr_attention_forward(const equigspr_attention* desc, void* out, void* out_low, float* lse, float* work, void* stream);
+/* out, out_low (may be null: out is then taken as exact), lse: as the forward wrote them; grad_q / grad_k / grad_v: contiguous, written (not accumulated), each may be null.
  * No atomics: results do not depend on timing. */
 int64_t equigspr_attention_backward_work_size(const equigspr_attention* desc);
-int equigspr_attention_backward(const equigspr_attention* desc, const void* out, const float* lse, const equigspr_attention_tensor* grad_out,
+int equigspr_attention_backward(const equigspr_attention* desc, const void* out, const void* out_low, const float* lse, const equigspr_attention_tensor* grad_out,
                                 float* work, void* grad_q, void* grad_k, void* grad_v, void* stream);
 
 #define EQUIGSPR_ACT_SILU 0
@@ -551,13 +551,13 @@ typedef struct equigspr_gated_feed_forward {
 typedef struct equigspr_gated_feed_forward_grads {
     void *grad_x, *grad_w_gate_up, *grad_w_down, *grad_b_gate_up, *grad_b_down;
 } equigspr_gated_feed_forward_grads;
-/* y [rows, out]; h [rows, hidden] (inputs' dtype): act(z) * u, kept for the backward; zu [rows, 2 * hidden] or null: both projections, likewise;
+/* y [rows, out]; h [rows, hidden] (inputs' dtype): act(z) * u, kept for the backward; zu [rows, 2 * hidden] floats or null: both projections, likewise;
  * work: ..._work_size floats (0: may be null) */
 int64_t equigspr_gated_feed_forward_work_size(const equigspr_gated_feed_forward* desc);
-int equigspr_gated_feed_forward_forward(const equigspr_gated_feed_forward* desc, void* y, void* h, void* zu, float* work, void* stream);
+int equigspr_gated_feed_forward_forward(const equigspr_gated_feed_forward* desc, void* y, void* h, float* zu, float* work, void* stream);
 /* grad_y [rows, out] contiguous; zu and h as the forward wrote them; dzu [rows, 2 * hidden]: scratch of the inputs' dtype */
 int64_t equigspr_gated_feed_forward_backward_work_size(const equigspr_gated_feed_forward* desc);
-int equigspr_gated_feed_forward_backward(const equigspr_gated_feed_forward* desc, const void* grad_y, const void* zu, const void* h, void* dzu, float* work,
+int equigspr_gated_feed_forward_backward(const equigspr_gated_feed_forward* desc, const void* grad_y, const float* zu, const void* h, void* dzu, float* work,
                                          const equigspr_gated_feed_forward_grads* grads, void* stream);
 
 /* The residual step between two blocks, with the norm behind the first and the norm before the second:

@@ -58,7 +58,7 @@ def attention(q, k, v, grad=None, q_lens=None, kv_lens=None, key_mask=None, caus
     dS = P * (dP - delta)
     p16 = u if dt != torch.float32 else 0.0
     e_p = (2 * rel + p16) * P                                                # error of a probability
-    e_dp = acc * (G.abs() @ V.abs().mT) + (G.abs() * (o_err + 4 * F32 * O.abs())).sum(-1, keepdim=True) + acc * (G.abs() * O.abs()).sum(-1, keepdim=True)
+    e_dp = acc * (G.abs() @ V.abs().mT) + (G.abs() * (o_err - u * O.abs() * (dt != torch.float32) + 4 * F32 * O.abs())).sum(-1, keepdim=True) + acc * (G.abs() * O.abs()).sum(-1, keepdim=True)
     if dt == torch.float16 and nk:
         # fp16 holds 2^E dS with 30000 <= 2^E bound <= 60000, bound = 2 d max|dO| max|V| (a power of two below 60000 / bound): below fp16's
         # normal range one rounding is off by up to half of its smallest step, 2^-25, which is 2^-25 2^-E <= 2^-25 bound / 30000 of dS.
@@ -111,8 +111,8 @@ def feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, g
         p16, pl = (u if dt != torch.float32 else 0.0), PLANES[dt]
         acc = lambda n: (n ** 0.5 * 2 + 8) * F32 + pl  # noqa: E731     sums of n products: 2 sqrt(n) roundings, 6 sigma of a random walk
         X, Wg, Wu, Wd = (leaf[n].abs() for n in names[:4])
-        e_z = acc(width) * (X @ Wg.mT + z.abs()) + p16 * z.abs()             # p16: z and u are kept in the inputs' type for the backward
-        e_u = acc(width) * (X @ Wu.mT + up.abs()) + p16 * up.abs()
+        e_z = acc(width) * (X @ Wg.mT + z.abs())
+        e_u = acc(width) * (X @ Wu.mT + up.abs())
         a = _act(activation, z)
         zz = z.detach().clone().requires_grad_(True)
         with torch.enable_grad():

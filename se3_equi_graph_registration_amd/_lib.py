@@ -148,9 +148,9 @@ _SIGNATURES = {
     "equigspr_match_descriptors": (ctypes.c_int, [c_void_p, c_int32, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
     "equigspr_correspondence_labels": (ctypes.c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p, ctypes.c_float, c_void_p, c_void_p, c_void_p]),
     "equigspr_attention_work_size": (c_int64, [POINTER(Attention)]),
-    "equigspr_attention_forward": (ctypes.c_int, [POINTER(Attention)] + [c_void_p] * 4),
+    "equigspr_attention_forward": (ctypes.c_int, [POINTER(Attention)] + [c_void_p] * 5),
     "equigspr_attention_backward_work_size": (c_int64, [POINTER(Attention)]),
-    "equigspr_attention_backward": (ctypes.c_int, [POINTER(Attention), c_void_p, c_void_p, POINTER(AttentionTensor)] + [c_void_p] * 5),
+    "equigspr_attention_backward": (ctypes.c_int, [POINTER(Attention), c_void_p, c_void_p, c_void_p, POINTER(AttentionTensor)] + [c_void_p] * 5),
     "equigspr_gated_feed_forward_work_size": (c_int64, [POINTER(GatedFeedForward)]),
     "equigspr_gated_feed_forward_forward": (ctypes.c_int, [POINTER(GatedFeedForward)] + [c_void_p] * 5),
     "equigspr_gated_feed_forward_backward_work_size": (c_int64, [POINTER(GatedFeedForward)]),

@@ -37,7 +37,7 @@ def _describe(q, k, v, q_lens, kv_lens, key_mask, causal, scale):
                           None if key_mask is None else key_mask.data_ptr(), 0 if key_mask is None else key_mask.stride(0))
 
 
-def _forward(q, k, v, q_lens, kv_lens, key_mask, causal, scale, want_lse):
+def _forward(q, k, v, q_lens, kv_lens, key_mask, causal, scale, training):
     L = _lib.lib()
     b, nq, h, d = q.shape
     with on_device(q.device):
@@ -45,9 +45,10 @@ def _forward(q, k, v, q_lens, kv_lens, key_mask, causal, scale, want_lse):
         n = L.equigspr_attention_work_size(ctypes.byref(desc))
         work = torch.empty(n, dtype=torch.float32, device=q.device) if n > 0 else None
         out = torch.empty((b, nq, h, d), dtype=q.dtype, device=q.device)
-        lse = torch.empty(b * h * nq, dtype=torch.float32, device=q.device) if want_lse else None
-        _lib.check(L.equigspr_attention_forward(ctypes.byref(desc), _p(out), _p(lse), _p(work), _stream()), "attention_forward")
-    return out, lse
+        low = torch.empty_like(out) if training and q.dtype != torch.float32 else None
+        lse = torch.empty(b * h * nq, dtype=torch.float32, device=q.device) if training else None
+        _lib.check(L.equigspr_attention_forward(ctypes.byref(desc), _p(out), _p(low), _p(lse), _p(work), _stream()), "attention_forward")
+    return out, low, lse
 
 
 class _AttentionFn(torch.autograd.Function):
@@ -55,15 +56,15 @@ class _AttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, q_lens, kv_lens, key_mask, causal, scale):
-        out, lse = _forward(q, k, v, q_lens, kv_lens, key_mask, causal, scale, True)
-        ctx.save_for_backward(q, k, v, q_lens, kv_lens, key_mask, out, lse)
+        out, low, lse = _forward(q, k, v, q_lens, kv_lens, key_mask, causal, scale, True)
+        ctx.save_for_backward(q, k, v, q_lens, kv_lens, key_mask, out, low, lse)
         ctx.causal, ctx.scale = causal, scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, q_lens, kv_lens, key_mask, out, lse = ctx.saved_tensors
+        q, k, v, q_lens, kv_lens, key_mask, out, low, lse = ctx.saved_tensors
         L = _lib.lib()
         need = ctx.needs_input_grad
         with on_device(q.device):
@@ -72,7 +73,7 @@ class _AttentionFn(torch.autograd.Function):
             gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else None for t, n in zip((q, k, v), need))
             work = torch.empty(L.equigspr_attention_backward_work_size(ctypes.byref(desc)), dtype=torch.float32, device=q.device)
             g = _tensor(grad)
-            _lib.check(L.equigspr_attention_backward(ctypes.byref(desc), _p(out), _p(lse), ctypes.byref(g), _p(work), _p(gq), _p(gk), _p(gv),
+            _lib.check(L.equigspr_attention_backward(ctypes.byref(desc), _p(out), _p(low), _p(lse), ctypes.byref(g), _p(work), _p(gq), _p(gk), _p(gv),
                                                      _stream()), "attention_backward")
         return gq, gk, gv, None, None, None, None, None
 

@@ -16,11 +16,23 @@ struct AttnFwd {
     AttnShape s;
     AttnTensor<T> q, k, v;
     typename Num<T>::type* out;               // [batch, nq, heads, dim] contiguous
+    typename Num<T>::type* out_low;           // 16-bit types, for the backward: what out's rounding dropped, or null
     float* lse;                               // [batch, kv_heads, nq * group] base-2 log-sum of the scaled scores, +inf for a row without keys
     int row_tiles, splits, split_keys;
     float* part_o;                            // [splits][batch * kv_heads][nq * group][dim]
     float* part_l;                            // [splits][batch * kv_heads][nq * group], -inf for a part without keys
 };
+
+template <int T>
+__device__ __forceinline__ void attn_store_out(typename Num<T>::type* out, typename Num<T>::type* low, const float (&x)[4], int n) {
+    store4<T>(out, x, n);
+    if (T != kF32 && low) {
+        float r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = x[i] - (float)(typename Num<T>::type)x[i];
+        store4<T>(low, r, n);
+    }
+}
 
 // W: width of the staged tiles, KS: steps of 16 that the head dim takes in them
 template <int T, int W, int KS, int NW>
@@ -172,7 +184,7 @@ __global__ __launch_bounds__(NW * 64, W == 128 && T == kF32 ? 1 : 2) void attn_f
     }
     if (a.lse && half == 0) a.lse[at] = lse;
     const int i0 = row_point(s, row);
-    typename Num<T>::type* o = a.out + (((int64_t)b * s.nq + i0) * s.heads + hk * s.group + row - i0 * s.group) * s.dim;
+    const int64_t o = (((int64_t)b * s.nq + i0) * s.heads + hk * s.group + row - i0 * s.group) * s.dim;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -181,7 +193,7 @@ __global__ __launch_bounds__(NW * 64, W == 128 && T == kF32 ? 1 : 2) void attn_f
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = exists ? acc[d][4 * g + i] * inv : 0.f;
-            store4<T>(o + c, x, s.dim - c);
+            attn_store_out<T>(a.out + o + c, a.out_low ? a.out_low + o + c : nullptr, x, s.dim - c);
         }
 }
 
@@ -211,7 +223,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnFwd<T> a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= inv;
     const int i0 = row_point(s, row);
-    store4<T>(a.out + (((int64_t)b * s.nq + i0) * s.heads + hk * s.group + row - i0 * s.group) * s.dim + c, v, left);
+    const int64_t o = (((int64_t)b * s.nq + i0) * s.heads + hk * s.group + row - i0 * s.group) * s.dim + c;
+    attn_store_out<T>(a.out + o, a.out_low ? a.out_low + o : nullptr, v, left);
 }
 
 // Rows of a workgroup: 128 (four waves share every key tile), or 32 when there are no more rows than that per key head (single tokens).
@@ -240,7 +253,7 @@ static int attn_fwd_launch(const AttnFwd<T>& a, int waves, int64_t blocks, hipSt
 }
 
 template <int T>
-static int attn_fwd(const equigspr_attention* d, const AttnShape& s, void* out, float* lse, float* work, hipStream_t st) {
+static int attn_fwd(const equigspr_attention* d, const AttnShape& s, void* out, void* out_low, float* lse, float* work, hipStream_t st) {
     using E = typename Num<T>::type;
     AttnFwd<T> a;
     a.s = s;
@@ -248,6 +261,7 @@ static int attn_fwd(const equigspr_attention* d, const AttnShape& s, void* out, 
     a.k = attn_tensor<T>(d->k, s.dim);
     a.v = attn_tensor<T>(d->v, s.dim);
     a.out = (E*)out;
+    a.out_low = (E*)out_low;
     a.lse = lse;
     const AttnPlan p = attn_plan(T, s.batch, s.nq, s.nk, s.heads, s.kv_heads);
     a.row_tiles = p.row_tiles; a.splits = p.splits; a.split_keys = p.split_keys;
@@ -297,7 +311,7 @@ extern "C" int64_t equigspr_attention_work_size(const equigspr_attention* d) {
     return (p.splits * n + 3) / 4 * 4 + p.splits * n * s.dim;
 }
 
-extern "C" int equigspr_attention_forward(const equigspr_attention* d, void* out, float* lse, float* work, void* stream) {
+extern "C" int equigspr_attention_forward(const equigspr_attention* d, void* out, void* out_low, float* lse, float* work, void* stream) {
     eq::AttnShape s;
     if (const int rc = eq::attn_shape(d, &s)) return rc;
     EQ_CHECK_ARG(out || !s.batch || !s.nq, EQUIGSPR_EINVAL, "attention_forward: out is null");
@@ -305,8 +319,8 @@ extern "C" int equigspr_attention_forward(const equigspr_attention* d, void* out
     if (s.batch == 0 || s.nq == 0) return 0;
     hipStream_t st = (hipStream_t)stream;
     switch (d->dtype) {
-        case EQUIGSPR_F32: return eq::attn_fwd<eq::kF32>(d, s, out, lse, work, st);
-        case EQUIGSPR_BF16: return eq::attn_fwd<eq::kBF16>(d, s, out, lse, work, st);
-        default: return eq::attn_fwd<eq::kF16>(d, s, out, lse, work, st);
+        case EQUIGSPR_F32: return eq::attn_fwd<eq::kF32>(d, s, out, out_low, lse, work, st);
+        case EQUIGSPR_BF16: return eq::attn_fwd<eq::kBF16>(d, s, out, out_low, lse, work, st);
+        default: return eq::attn_fwd<eq::kF16>(d, s, out, out_low, lse, work, st);
     }
 }

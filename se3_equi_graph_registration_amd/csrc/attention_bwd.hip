@@ -4,7 +4,8 @@
 // attn_dkv_kernel owns 32 keys per wave and walks the packed rows -- all query heads of the group, so the gradients of shared keys need
 // no atomics and do not depend on timing.  In each, the score tile is formed with the owned index in the lane, which makes P and dS the
 // B operands of the products that follow as they stand (see attention.hip); the other operand is the staged tile read transposed.
-// P and dS are rounded to the inputs' 16-bit type for those products, everything else is fp32.
+// P and dS are rounded to the inputs' 16-bit type for those products, everything else is fp32; the forward leaves what the output's
+// rounding dropped in a second plane for delta, whose error every dS of the row would share.
 // fp16: dS is about 1/keys of the output gradient and would sink below fp16's range, so it is held as 2^E dS, with E from the largest
 // |dO| and |V| such that the bound |dS| <= 2 dim max|dO| max|V| stays in range; undone in fp32 at the end.
 #include "attention_device.h"
@@ -17,6 +18,7 @@ template <int T>
 struct AttnBwd {
     AttnShape s;
     AttnTensor<T> q, k, v, o, g;              // g: gradient of the output
+    const typename Num<T>::type* o_low;       // 16-bit types: what the output's rounding dropped, or null
     const float* lse;
     float* delta;                             // [batch, kv_heads, nq * group]
     float* amax;                              // fp16: [2 * kAmaxBlocks]
@@ -120,6 +122,11 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_ker
             const Raw8<T> rg = ok_row ? load8<T>(pg, c, s.dim) : raw_zero<T>(), ro = ok_row ? load8<T>(po, c, s.dim) : raw_zero<T>();
 #pragma unroll
             for (int i = 0; i < 8; ++i) delta = fmaf(raw_float<T>(rg, i), raw_float<T>(ro, i), delta);
+            if (T != kF32 && a.o_low && ok_row) {
+                const Raw8<T> rl = load8<T>(a.o_low + (po - a.o.p), c, s.dim);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) delta = fmaf(raw_float<T>(rg, i), raw_float<T>(rl, i), delta);
+            }
             g[ks] = planes_of<T>(rg);
         }
     }
@@ -437,8 +444,8 @@ static int attn_bwd_launch(const AttnBwd<T>& a, hipStream_t st) {
 }
 
 template <int T>
-static int attn_bwd(const equigspr_attention* d, const AttnShape& s, const void* out, const float* lse, const equigspr_attention_tensor* grad_out,
-                    float* work, void* gq, void* gk, void* gv, hipStream_t st) {
+static int attn_bwd(const equigspr_attention* d, const AttnShape& s, const void* out, const void* out_low, const float* lse,
+                    const equigspr_attention_tensor* grad_out, float* work, void* gq, void* gk, void* gv, hipStream_t st) {
     using E = typename Num<T>::type;
     AttnBwd<T> a;
     a.s = s;
@@ -448,6 +455,7 @@ static int attn_bwd(const equigspr_attention* d, const AttnShape& s, const void*
     a.g = attn_tensor<T>(*grad_out, s.dim);
     const equigspr_attention_tensor o = {const_cast<void*>(out), (int64_t)s.nq * s.heads * s.dim, (int64_t)s.heads * s.dim, s.dim};
     a.o = attn_tensor<T>(o, s.dim);
+    a.o_low = (const E*)out_low;
     a.lse = lse;
     a.amax = work;
     const AttnBwdPlan p = attn_bwd_plan(s);
@@ -468,8 +476,8 @@ extern "C" int64_t equigspr_attention_backward_work_size(const equigspr_attentio
     return 2 * eq::kAmaxBlocks + p.delta + (p.parts_q > 2 * p.parts_k ? p.parts_q : 2 * p.parts_k);
 }
 
-extern "C" int equigspr_attention_backward(const equigspr_attention* d, const void* out, const float* lse, const equigspr_attention_tensor* grad_out,
-                                           float* work, void* grad_q, void* grad_k, void* grad_v, void* stream) {
+extern "C" int equigspr_attention_backward(const equigspr_attention* d, const void* out, const void* out_low, const float* lse,
+                                           const equigspr_attention_tensor* grad_out, float* work, void* grad_q, void* grad_k, void* grad_v, void* stream) {
     eq::AttnShape s;
     if (const int rc = eq::attn_shape(d, &s)) return rc;
     EQ_CHECK_ARG(grad_out && work, EQUIGSPR_EINVAL, "attention_backward: grad_out or work is null");
@@ -478,8 +486,8 @@ extern "C" int equigspr_attention_backward(const equigspr_attention* d, const vo
     if (s.batch == 0) return 0;
     hipStream_t st = (hipStream_t)stream;
     switch (d->dtype) {
-        case EQUIGSPR_F32: return eq::attn_bwd<eq::kF32>(d, s, out, lse, grad_out, work, grad_q, grad_k, grad_v, st);
-        case EQUIGSPR_BF16: return eq::attn_bwd<eq::kBF16>(d, s, out, lse, grad_out, work, grad_q, grad_k, grad_v, st);
-        default: return eq::attn_bwd<eq::kF16>(d, s, out, lse, grad_out, work, grad_q, grad_k, grad_v, st);
+        case EQUIGSPR_F32: return eq::attn_bwd<eq::kF32>(d, s, out, out_low, lse, grad_out, work, grad_q, grad_k, grad_v, st);
+        case EQUIGSPR_BF16: return eq::attn_bwd<eq::kBF16>(d, s, out, out_low, lse, grad_out, work, grad_q, grad_k, grad_v, st);
+        default: return eq::attn_bwd<eq::kF16>(d, s, out, out_low, lse, grad_out, work, grad_q, grad_k, grad_v, st);
     }
 }

@@ -6,8 +6,9 @@
 //   kPlain  C = A B^T (+ bias), or fp32 partial tiles of a cut contraction, summed in order by ff_sum_kernel
 // z | u and dz | du are [rows, 2 hidden]: dx is ONE product over 2 hidden, dWg and dWu are the two halves of ONE product's rows.
 // A product's operands may run along or across the contraction in memory; across, the tile is read transposed (planes.h), so nothing
-// is ever transposed in memory.  Products accumulate in fp32; h, z, u, dz, du are stored in the inputs' type (what a 16-bit program
-// keeps between its layers: one rounding each), fp32 inputs stay fp32 with three-plane products.
+// is ever transposed in memory.  Products accumulate in fp32.  h, dz and du are operands of further products and are stored in the
+// inputs' type (one rounding each); z | u, which only the epilogue of the backward reads, stays fp32 -- in 16 bits its rounding would come
+// on top of dz's and du's in every gradient (bf16: 1.8 instead of 1.4 times the outputs' own rounding).
 // Bound: the matrix pipe for many rows, the weights' bytes for few.
 #include "planes.h"
 
@@ -36,7 +37,7 @@ struct FfArgs {
     E* c;                                     // [m, n]
     const E *bias, *bias2;
     float* part;                              // [cuts][m][n]
-    E* zu;                                    // kGate: written if not null; kGrad: read.  [m, 2 n]
+    float* zu;                                // kGate: written if not null; kGrad: read.  [m, 2 n]
     E* dzu;                                   // kGrad: [m, 2 n]
     int act;
 };
@@ -280,13 +281,13 @@ __global__ __launch_bounds__((FfShapeOf<T, kLarge>::kThreads), 2) void ff_produc
                 }
                 store8<T>(g.c + (int64_t)row * g.n + col, h, left);
                 if (g.zu) {
-                    store8<T>(g.zu + (int64_t)row * 2 * g.n + col, z, left);
-                    store8<T>(g.zu + (int64_t)row * 2 * g.n + g.n + col, u, left);
+                    store8<kF32>(g.zu + (int64_t)row * 2 * g.n + col, z, left);
+                    store8<kF32>(g.zu + (int64_t)row * 2 * g.n + g.n + col, u, left);
                 }
             } else if constexpr (kEpi == kGrad) {
                 const int64_t at = (int64_t)row * 2 * g.n + col;
-                load8f<T>(g.zu + at, left, z);
-                load8f<T>(g.zu + at + g.n, left, u);
+                load8f<kF32>(g.zu + at, left, z);
+                load8f<kF32>(g.zu + at + g.n, left, u);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float a, d;
@@ -406,8 +407,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void ff_few_kernel(FfArgs<T> g) {
         }
         store4<T>(g.c + (int64_t)row * g.n + col, h, left);
         if (g.zu) {
-            store4<T>(g.zu + (int64_t)row * 2 * g.n + col, v[0], left);
-            store4<T>(g.zu + (int64_t)row * 2 * g.n + g.n + col, v[1], left);
+            store4<kF32>(g.zu + (int64_t)row * 2 * g.n + col, v[0], left);
+            store4<kF32>(g.zu + (int64_t)row * 2 * g.n + g.n + col, v[1], left);
         }
     } else {
         store4<T>(g.c + (int64_t)row * g.n + col, v[0], left);
@@ -544,7 +545,7 @@ static FfOperand<T> ff_operand(const void* p, int rows, int len) {
 }
 
 template <int T>
-static int ff_forward(const equigspr_gated_feed_forward* d, void* y, void* h, void* zu, float* work, hipStream_t st) {
+static int ff_forward(const equigspr_gated_feed_forward* d, void* y, void* h, float* zu, float* work, hipStream_t st) {
     using E = typename Num<T>::type;
     FfArgs<T> g = {};
     g.act = d->activation;
@@ -553,7 +554,7 @@ static int ff_forward(const equigspr_gated_feed_forward* d, void* y, void* h, vo
     g.b.q = (const E*)d->w_up;
     g.m = d->rows; g.n = d->hidden; g.k = d->width;
     g.bias = (const E*)d->b_gate; g.bias2 = (const E*)d->b_up;
-    g.c = (E*)h; g.zu = (E*)zu;
+    g.c = (E*)h; g.zu = zu;
     const bool few = d->rows <= kFewRows;
     if (const int rc = few ? ff_few<T, kGate>(g, st, "gated_feed_forward (projections)") : ff_product<T, false, false, kGate>(g, st, "gated_feed_forward (projections)"))
         return rc;
@@ -566,7 +567,7 @@ static int ff_forward(const equigspr_gated_feed_forward* d, void* y, void* h, vo
 }
 
 template <int T>
-static int ff_backward(const equigspr_gated_feed_forward* d, const void* gy, const void* zu, const void* h, void* dzu, float* work,
+static int ff_backward(const equigspr_gated_feed_forward* d, const void* gy, const float* zu, const void* h, void* dzu, float* work,
                        const equigspr_gated_feed_forward_grads* o, hipStream_t st) {
     using E = typename Num<T>::type;
     const int r = d->rows, w = d->width, hd = d->hidden, out = d->out;
@@ -576,9 +577,10 @@ static int ff_backward(const equigspr_gated_feed_forward* d, const void* gy, con
     g.a = ff_operand<T>(gy, r, out);
     g.b = ff_operand<T>(d->w_down, out, hd);
     g.m = r; g.n = hd; g.k = out;
-    g.zu = (E*)const_cast<void*>(zu); g.dzu = (E*)dzu;
+    g.zu = const_cast<float*>(zu); g.dzu = (E*)dzu;
     if (const int rc = ff_product<T, false, true, kGrad>(g, st, "gated_feed_forward_backward (hidden)")) return rc;
-    g.zu = g.dzu = nullptr;
+    g.zu = nullptr;
+    g.dzu = nullptr;
     g.part = work;
     if (o->grad_x) {                          // [dz | du] [Wg ; Wu]
         g.a = ff_operand<T>(dzu, r, 2 * hd);
@@ -631,7 +633,7 @@ extern "C" int64_t equigspr_gated_feed_forward_work_size(const equigspr_gated_fe
     return d->rows <= eq::kFewRows ? 0 : eq::ff_part_size(d->dtype, d->rows, d->out, d->hidden);
 }
 
-extern "C" int equigspr_gated_feed_forward_forward(const equigspr_gated_feed_forward* d, void* y, void* h, void* zu, float* work, void* stream) {
+extern "C" int equigspr_gated_feed_forward_forward(const equigspr_gated_feed_forward* d, void* y, void* h, float* zu, float* work, void* stream) {
     if (const int rc = eq::ff_check(d)) return rc;
     if (d->rows == 0) return 0;
     EQ_CHECK_ARG(y && h && (work || equigspr_gated_feed_forward_work_size(d) == 0), EQUIGSPR_EINVAL, "gated_feed_forward_forward: null output or work");
@@ -653,7 +655,7 @@ extern "C" int64_t equigspr_gated_feed_forward_backward_work_size(const equigspr
     return sums > n ? sums : n;
 }
 
-extern "C" int equigspr_gated_feed_forward_backward(const equigspr_gated_feed_forward* d, const void* grad_y, const void* zu, const void* h, void* dzu, float* work,
+extern "C" int equigspr_gated_feed_forward_backward(const equigspr_gated_feed_forward* d, const void* grad_y, const float* zu, const void* h, void* dzu, float* work,
                                                     const equigspr_gated_feed_forward_grads* grads, void* stream) {
     if (const int rc = eq::ff_check(d)) return rc;
     if (d->rows == 0) return 0;

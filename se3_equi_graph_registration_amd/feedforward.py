@@ -29,7 +29,8 @@ def _forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, training):
         desc = _describe(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
         n = L.equigspr_gated_feed_forward_work_size(ctypes.byref(desc))
         work = torch.empty(n, dtype=torch.float32, device=x.device) if n > 0 else None
-        y, h, zu = new(rows, w_down.shape[0]), new(rows, hidden), new(rows, 2 * hidden) if training else None
+        y, h = new(rows, w_down.shape[0]), new(rows, hidden)
+        zu = torch.empty(rows, 2 * hidden, dtype=torch.float32, device=x.device) if training else None
         _lib.check(L.equigspr_gated_feed_forward_forward(ctypes.byref(desc), _p(y), _p(h), _p(zu), _p(work), _stream()),
                    "gated_feed_forward_forward")
     return y, zu, h
@@ -79,7 +80,8 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
     ``x [..., width]``, ``w_gate`` and ``w_up [hidden, width]``, ``w_down [out, hidden]`` (the layout of ``nn.Linear``), biases optional:
     float32, bfloat16 or float16, all alike, on one device (tensors that are not contiguous are copied).  ``activation``: "silu", "gelu"
     (exact) or "relu".  Products accumulate in fp32; the hidden layer is held in the inputs' dtype between the two products, as are the
-    two projections and their gradients in the backward: in float16 they must stay within that type's range.  Differentiable once in every tensor; bitwise
+    projections' gradients in the backward: in float16 they must stay within that type's range.  The backward keeps both projections in
+    float32.  Differentiable once in every tensor; bitwise
     reproducible (no atomics)."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"gated_feed_forward: activation {activation!r}, expected one of {sorted(ACTIVATIONS)}")

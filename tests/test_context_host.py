@@ -48,21 +48,21 @@ def test_attention_entry_refuses(over, code):
     d = _attention(**over)
     assert L.equigspr_attention_work_size(ctypes.byref(d)) == -1
     assert L.equigspr_attention_backward_work_size(ctypes.byref(d)) == -1
-    assert L.equigspr_attention_forward(ctypes.byref(d), 16, None, None, None) == code
-    assert L.equigspr_attention_backward(ctypes.byref(d), 16, 16, ctypes.byref(d.q), 16, None, None, None, None) == code
+    assert L.equigspr_attention_forward(ctypes.byref(d), 16, None, None, None, None) == code
+    assert L.equigspr_attention_backward(ctypes.byref(d), 16, None, 16, ctypes.byref(d.q), 16, None, None, None, None) == code
     assert L.equigspr_last_error()
 
 
 def test_entries_refuse_null_pointers_and_bad_sizes():
     L = _lib.lib()
     d = _attention()
-    assert L.equigspr_attention_forward(None, 16, None, None, None) == -1
-    assert L.equigspr_attention_forward(ctypes.byref(d), None, None, None, None) == -1
-    assert L.equigspr_attention_backward(ctypes.byref(d), 16, 16, None, 16, None, None, None, None) == -1
+    assert L.equigspr_attention_forward(None, 16, None, None, None, None) == -1
+    assert L.equigspr_attention_forward(ctypes.byref(d), None, None, None, None, None) == -1
+    assert L.equigspr_attention_backward(ctypes.byref(d), 16, None, 16, None, 16, None, None, None, None) == -1
     long = _attention(nq=1, nk=100000, batch=1, kv_heads=4)
     assert L.equigspr_attention_work_size(ctypes.byref(long)) > 0
-    assert L.equigspr_attention_forward(ctypes.byref(long), 16, None, None, None) == -1          # needs its workspace
-    assert L.equigspr_attention_forward(ctypes.byref(_attention(batch=0)), None, None, None, None) == 0
+    assert L.equigspr_attention_forward(ctypes.byref(long), 16, None, None, None, None) == -1          # needs its workspace
+    assert L.equigspr_attention_forward(ctypes.byref(_attention(batch=0)), None, None, None, None, None) == 0
     ff = dict(dtype=0, activation=0, rows=3, width=8, hidden=16, out=8, x=16, w_gate=16, w_up=16, w_down=16)
     for over in (dict(dtype=7), dict(activation=3), dict(rows=-1), dict(hidden=0), dict(x=None), dict(w_up=None)):
         f = _lib.GatedFeedForward(**{**ff, **over})
