@@ -5,77 +5,18 @@ Beside the local aggregation over k-NN neighbours (``EGNN``, ``GraphConvolution`
 points of its own cloud or of the other one.  No counterpart in the reference (its ``CrossAttentionPoseRegression`` holds no attention)."""
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
-from . import _lib
-from .ops import DTYPE_CODES, _p, _stream, check_capture, need_float, on_device, wants_grad
-
-
-def _stride(t, axis):
-    return t.stride(axis) if t.shape[axis] > 1 else 0
+from .ops import context_ops, need_float
 
 
 def _rows(t):
     """The kernels walk rows of unit stride, points and heads less than 2^31 / 128 bytes apart; any other stride is taken as it is."""
-    near = (_stride(t, 1) + _stride(t, 2)) * 128 * t.element_size() < 1 << 31
-    return t if near and (t.shape[-1] == 1 or t.stride(-1) == 1) else t.contiguous()
-
-
-def _tensor(t):
-    return _lib.AttentionTensor(t.data_ptr(), _stride(t, 0), _stride(t, 1), _stride(t, 2))
-
-
-def _describe(q, k, v, q_lens, kv_lens, key_mask, causal, scale):
-    b, nq, h, d = q.shape
-    return _lib.Attention(DTYPE_CODES[q.dtype], b, nq, k.shape[1], h, k.shape[2], d, int(causal), scale, _tensor(q), _tensor(k), _tensor(v),
-                          None if q_lens is None else q_lens.data_ptr(), None if kv_lens is None else kv_lens.data_ptr(),
-                          None if key_mask is None else key_mask.data_ptr(), 0 if key_mask is None else key_mask.stride(0))
-
-
-def _forward(q, k, v, q_lens, kv_lens, key_mask, causal, scale, training):
-    L = _lib.lib()
-    b, nq, h, d = q.shape
-    with on_device(q.device):
-        desc = _describe(q, k, v, q_lens, kv_lens, key_mask, causal, scale)
-        n = L.equigspr_attention_work_size(ctypes.byref(desc))
-        work = torch.empty(n, dtype=torch.float32, device=q.device) if n > 0 else None
-        out = torch.empty((b, nq, h, d), dtype=q.dtype, device=q.device)
-        low = torch.empty_like(out) if training and q.dtype != torch.float32 else None
-        lse = torch.empty(b * h * nq, dtype=torch.float32, device=q.device) if training else None
-        _lib.check(L.equigspr_attention_forward(ctypes.byref(desc), _p(out), _p(low), _p(lse), _p(work), _stream()), "attention_forward")
-    return out, low, lse
-
-
-class _AttentionFn(torch.autograd.Function):
-    """``equigspr_attention_forward`` / ``_backward``: the probabilities are recomputed from the rows' log-sums."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, q_lens, kv_lens, key_mask, causal, scale):
-        out, low, lse = _forward(q, k, v, q_lens, kv_lens, key_mask, causal, scale, True)
-        ctx.save_for_backward(q, k, v, q_lens, kv_lens, key_mask, out, low, lse)
-        ctx.causal, ctx.scale = causal, scale
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        q, k, v, q_lens, kv_lens, key_mask, out, low, lse = ctx.saved_tensors
-        L = _lib.lib()
-        need = ctx.needs_input_grad
-        with on_device(q.device):
-            grad = _rows(grad)
-            desc = _describe(q, k, v, q_lens, kv_lens, key_mask, ctx.causal, ctx.scale)
-            gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else None for t, n in zip((q, k, v), need))
-            work = torch.empty(L.equigspr_attention_backward_work_size(ctypes.byref(desc)), dtype=torch.float32, device=q.device)
-            g = _tensor(grad)
-            _lib.check(L.equigspr_attention_backward(ctypes.byref(desc), _p(out), _p(low), _p(lse), ctypes.byref(g), _p(work), _p(gq), _p(gk), _p(gv),
-                                                     _stream()), "attention_backward")
-        return gq, gk, gv, None, None, None, None, None
+    n, m = t.stride(1) if t.shape[1] > 1 else 0, t.stride(2) if t.shape[2] > 1 else 0
+    return t if (n + m) * 128 * t.element_size() < 1 << 31 and (t.shape[-1] == 1 or t.stride(-1) == 1) else t.contiguous()
 
 
 def _need_lens(t, name, q):
@@ -122,11 +63,7 @@ def cloud_attention(q, k, v, *, q_lens=None, kv_lens=None, key_mask=None, causal
                                f"on {key_mask.device}")
         if key_mask.shape[1] > 1 and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    if wants_grad(q, k, v):
-        check_capture(q, k, v)
-        return _AttentionFn.apply(q, k, v, q_lens, kv_lens, key_mask, bool(causal), scale)
-    return _forward(q, k, v, q_lens, kv_lens, key_mask, bool(causal), scale, False)[0]
+    return context_ops().cloud_attention(_rows(q), _rows(k), _rows(v), q_lens, kv_lens, key_mask, bool(causal), scale)
 
 
 class CloudAttention(nn.Module):

@@ -5,7 +5,6 @@
 // ends, and there is exactly one implementation underneath.  Built by csrc/Makefile into ../libequigspr_torch.so (g++; no device
 // code here) and loaded with torch.ops.load_library (se3_equi_graph_registration_amd/torch_library.py).
 #include <ATen/ATen.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/autograd.h>
@@ -515,26 +514,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> irrep_conv_forward_autograd(const
     auto out = IrrepConvFn::apply(f0, f1, x, row, col, w_r1, b_r1, w_r2, b_r2, ws0, ws1, basis.vec());
     return {out[0], out[1], out[2]};
 }
-// Whether a backward that is recorded into a hipGraph from here on would reach into work of another stream: `t` belongs to an autograd graph
-// -- or, a leaf, hangs on the gradient accumulator of one -- that was built on a stream that is not being captured.  The autograd engine
-// would synchronise with that stream during the capture, which ends the process; the callers raise instead.
-bool grad_lives_on_other_stream(const at::Tensor& t) {
-    if (!t.is_cuda() || !t.requires_grad()) return false;
-    const std::shared_ptr<torch::autograd::Node> node = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
-    if (!node) return false;
-    const auto stream = node->stream();
-    if (!stream.has_value()) return false;
-    const c10::hip::HIPStreamMasqueradingAsCUDA other(*stream);      // autograd's streams carry the masqueraded device type
-    if (other.stream() == cur_stream(t)) return false;
-    if (other.stream() == nullptr) return true;                 // the default stream is never part of a capture
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(other.stream(), &status) != hipSuccess) { (void)hipGetLastError(); return true; }
-    return status != hipStreamCaptureStatusActive;
-}
 }  // namespace
 
 TORCH_LIBRARY(equigspr, m) {
-    m.def("grad_lives_on_other_stream(Tensor t) -> bool", &grad_lives_on_other_stream);
     m.def("abi_version() -> int", &abi_version);
     m.def("knn_graph(Tensor x, int k, bool loop=True) -> Tensor");
     m.def("build_inverse_index(Tensor key, int n_nodes) -> (Tensor, Tensor, Tensor)");

@@ -3,75 +3,11 @@ layer with its parameters.  Stands beside the two-Linear MLPs of ``E_GCL``, ``SO
 compiled for their narrow widths."""
 from __future__ import annotations
 
-import ctypes
-
-import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
-from . import _lib
-from .ops import DTYPE_CODES, _p, _stream, check_capture, need_float, on_device, wants_grad
+from .ops import context_ops, need_float
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}      # EQUIGSPR_ACT_*
-
-
-def _describe(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act):
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    return _lib.GatedFeedForward(DTYPE_CODES[x.dtype], act, x.shape[0], x.shape[1], w_gate.shape[0], w_down.shape[0], ptr(x), ptr(w_gate),
-                                 ptr(w_up), ptr(w_down), ptr(b_gate), ptr(b_up), ptr(b_down))
-
-
-def _forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, training):
-    L = _lib.lib()
-    new = lambda *s: torch.empty(s, dtype=x.dtype, device=x.device)  # noqa: E731
-    rows, hidden = x.shape[0], w_gate.shape[0]
-    with on_device(x.device):
-        desc = _describe(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
-        n = L.equigspr_gated_feed_forward_work_size(ctypes.byref(desc))
-        work = torch.empty(n, dtype=torch.float32, device=x.device) if n > 0 else None
-        y, h = new(rows, w_down.shape[0]), new(rows, hidden)
-        zu = torch.empty(rows, 2 * hidden, dtype=torch.float32, device=x.device) if training else None
-        _lib.check(L.equigspr_gated_feed_forward_forward(ctypes.byref(desc), _p(y), _p(h), _p(zu), _p(work), _stream()),
-                   "gated_feed_forward_forward")
-    return y, zu, h
-
-
-class _FeedForwardFn(torch.autograd.Function):
-    """``equigspr_gated_feed_forward_forward`` / ``_backward``; both projections and the hidden layer are kept."""
-
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act):
-        y, zu, h = _forward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, True)
-        ctx.save_for_backward(x, w_gate, w_up, w_down, zu, h)
-        ctx.act = act
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gy):
-        x, w_gate, w_up, w_down, zu, h = ctx.saved_tensors
-        L = _lib.lib()
-        need = ctx.needs_input_grad
-        rows, width = x.shape
-        hidden, out = w_gate.shape[0], w_down.shape[0]
-        make = torch.empty if rows else torch.zeros
-        new = lambda *s: make(s, dtype=x.dtype, device=x.device)  # noqa: E731
-        with on_device(x.device):
-            gy = gy.contiguous()
-            desc = _describe(x, w_gate, w_up, w_down, None, None, None, ctx.act)
-            gx = new(rows, width) if need[0] else None
-            gw = new(2 * hidden, width) if need[1] or need[2] else None
-            gd = new(out, hidden) if need[3] else None
-            gb = new(2 * hidden) if need[4] or need[5] else None
-            gbd = new(out) if need[6] else None
-            dzu = new(rows, 2 * hidden)
-            work = torch.empty(max(1, L.equigspr_gated_feed_forward_backward_work_size(ctypes.byref(desc))), dtype=torch.float32, device=x.device)
-            ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-            grads = _lib.GatedFeedForwardGrads(ptr(gx), ptr(gw), ptr(gd), ptr(gb), ptr(gbd))
-            _lib.check(L.equigspr_gated_feed_forward_backward(ctypes.byref(desc), _p(gy), _p(zu), _p(h), _p(dzu), _p(work), ctypes.byref(grads),
-                                                              _stream()), "gated_feed_forward_backward")
-        return (gx, gw[:hidden] if need[1] else None, gw[hidden:] if need[2] else None, gd, gb[:hidden] if need[4] else None,
-                gb[hidden:] if need[5] else None, gbd, None)
 
 
 def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, *, activation="silu"):
@@ -100,12 +36,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
             raise RuntimeError(f"{name}: expected [{n}], got {tuple(t.shape)}")
     args = [x.reshape(-1, width).contiguous(), w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()]
     args += [None if t is None else t.contiguous() for t in (b_gate, b_up, b_down)]
-    if wants_grad(*args):
-        check_capture(*args)
-        y = _FeedForwardFn.apply(*args, ACTIVATIONS[activation])
-    else:
-        y = _forward(*args, ACTIVATIONS[activation], False)[0]
-    return y.view(*x.shape[:-1], out)
+    return context_ops().gated_feed_forward(*args, ACTIVATIONS[activation]).view(*x.shape[:-1], out)
 
 
 class GatedFeedForward(nn.Module):

@@ -3,66 +3,13 @@ with its parameters.  The norm behind a block, its gate, the residual scale, the
 over memory (the ``LayerNorm`` of ``E_GCL`` lives inside the edge kernels and is not reachable on its own)."""
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
-from . import _lib
-from .ops import DTYPE_CODES, _p, _stream, check_capture, need_float, on_device, wants_grad
+from .ops import context_ops, need_float
 
-KINDS = {"layer": 0, "rms": 1}
+KINDS = ("layer", "rms")
 _MAX_WIDTH = 8192
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _describe(x, f, pre_w, pre_b, post_w, post_b, gate, scale, rms, eps, factor, gate_rows):
-    return _lib.ResidualNorm(DTYPE_CODES[x.dtype], x.shape[-1], rms, 0, x.numel() // x.shape[-1], gate_rows, eps, factor, _ptr(x), _ptr(f),
-                             _ptr(gate), _ptr(post_w), _ptr(post_b), _ptr(pre_w), _ptr(pre_b), _ptr(scale))
-
-
-def _forward(x, f, pre_w, pre_b, post_w, post_b, gate, scale, rms, eps, factor, gate_rows):
-    with on_device(x.device):
-        desc = _describe(x, f, pre_w, pre_b, post_w, post_b, gate, scale, rms, eps, factor, gate_rows)
-        y = torch.empty_like(x) if f is not None else None
-        u = torch.empty_like(x) if pre_w is not None else None
-        _lib.check(_lib.lib().equigspr_residual_norm_forward(ctypes.byref(desc), _p(y), _p(u), _stream()), "residual_norm_forward")
-    return y, u
-
-
-class _ResidualNormFn(torch.autograd.Function):
-    """``equigspr_residual_norm_forward`` / ``_backward``; nothing but the inputs is kept, the norms are recomputed."""
-
-    @staticmethod
-    def forward(ctx, x, f, pre_w, pre_b, post_w, post_b, gate, scale, rms, eps, factor, gate_rows):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, f, pre_w, pre_b, post_w, post_b, gate, scale)
-        ctx.rest = (rms, eps, factor, gate_rows)
-        return _forward(x, f, pre_w, pre_b, post_w, post_b, gate, scale, rms, eps, factor, gate_rows)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gy, gu):
-        saved = ctx.saved_tensors
-        x, f, pre_w, pre_b, post_w, post_b, gate, scale = saved
-        L = _lib.lib()
-        need = ctx.needs_input_grad
-        with on_device(x.device):
-            desc = _describe(*saved, *ctx.rest)
-            gy, gu = (None if g is None else g.contiguous() for g in (gy, gu))
-            make = torch.empty_like if x.numel() else torch.zeros_like
-            got = [make(t) if t is not None and n else None for t, n in zip(saved, need)]
-            gx, gf, gpre_w, gpre_b, gpost_w, gpost_b, ggate, gscale = got
-            n = L.equigspr_residual_norm_backward_work_size(ctypes.byref(desc))
-            work = torch.empty(max(1, n), dtype=torch.float32, device=x.device)
-            grads = _lib.ResidualNormGrads(_ptr(gx), _ptr(gf), _ptr(ggate), _ptr(gpost_w), _ptr(gpost_b), _ptr(gpre_w), _ptr(gpre_b), _ptr(gscale))
-            _lib.check(L.equigspr_residual_norm_backward(ctypes.byref(desc), _p(gy), _p(gu), _p(work), ctypes.byref(grads), _stream()),
-                       "residual_norm_backward")
-        return (*got, None, None, None, None)
 
 
 def residual_norm(x, f, pre_weight=None, pre_bias=None, *, post_weight=None, post_bias=None, gate=None, scale=None, kind="layer", eps=1e-5):
@@ -105,21 +52,14 @@ def residual_norm(x, f, pre_weight=None, pre_bias=None, *, post_weight=None, pos
     if scale is not None and not isinstance(scale, torch.Tensor):
         factor, scale = float(scale), None
     params = []
-    for t, name in ((pre_weight, "pre_weight"), (pre_bias, "pre_bias"), (post_weight, "post_weight"), (post_bias, "post_bias"), (scale, "scale")):
-        if t is not None:
+    for t, name in ((pre_weight, "pre_weight"), (pre_bias, "pre_bias"), (post_weight, "post_weight"), (post_bias, "post_bias"), (gate, "gate"), (scale, "scale")):
+        if t is not None and name != "gate":
             if need_float(t, name).shape != (c,) or t.device != x.device:
                 raise RuntimeError(f"{name}: expected [{c}] on {x.device}, got {tuple(t.shape)} on {t.device}")
             t = t.float().contiguous()
         params.append(t)
-    pre_weight, pre_bias, post_weight, post_bias, scale = params
-    args = (x.contiguous(), None if f is None else f.contiguous(), pre_weight, pre_bias, post_weight, post_bias, gate, scale)
-    rest = (KINDS[kind], eps, factor, gate_rows)
-    if wants_grad(*args):
-        check_capture(*args)
-        y, u = _ResidualNormFn.apply(*args, *rest)
-    else:
-        y, u = _forward(*args, *rest)
-    return (x if f is None else y), u
+    y, u = context_ops().residual_norm(x.contiguous(), None if f is None else f.contiguous(), *params, kind == "rms", eps, factor, gate_rows)
+    return (x if f is None else y), (None if pre_weight is None else u)
 
 
 class ResidualNorm(nn.Module):

@@ -39,7 +39,8 @@ def _stream():
 
 
 # ----------------------------------------------------------------------------------- operators of several element types
-DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # EQUIGSPR_F32 / EQUIGSPR_BF16 / EQUIGSPR_F16
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)      # EQUIGSPR_F32 / EQUIGSPR_BF16 / EQUIGSPR_F16
+_CONTEXT_OPS = None
 
 
 def need_float(t, name, like=None, ndim=None):
@@ -49,7 +50,7 @@ def need_float(t, name, like=None, ndim=None):
     if not t.is_cuda:
         raise RuntimeError(f"{name}: expected a tensor on the MI355X (cuda/HIP) device, got {t.device}; "
                            "this package has no CPU path")
-    if t.dtype not in DTYPE_CODES:
+    if t.dtype not in _FLOATS:
         raise RuntimeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
         raise RuntimeError(f"{name}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
@@ -58,36 +59,13 @@ def need_float(t, name, like=None, ndim=None):
     return t
 
 
-def wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def check_capture(*tensors):
-    """Refuses to record a differentiable call into a hipGraph when one of its inputs hangs on an autograd graph of another stream (an
-    eager graph of the same leaves that is still alive): the backward would synchronise with that stream during the capture."""
-    if not torch.cuda.is_current_stream_capturing():
-        return
-    from . import torch_library
-    other = torch_library.load().grad_lives_on_other_stream
-    for i, t in enumerate(tensors):
-        if t is not None and other(t):
-            raise RuntimeError(f"input {i} hangs on an autograd graph that was built on another stream and is still alive: drop that graph's "
-                               "outputs (or run it on the capturing stream) before recording this call into a hipGraph")
-
-
-class on_device:
-    """The call's tensors' device as the current one (a no-op where it already is)."""
-
-    def __init__(self, device):
-        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+def context_ops():
+    """``torch.ops.equigspr`` (csrc/torch_context_ops.cpp): the context operators with their autograd nodes."""
+    global _CONTEXT_OPS
+    if _CONTEXT_OPS is None:
+        from . import torch_library
+        _CONTEXT_OPS = torch_library.load()
+    return _CONTEXT_OPS
 
 
 EDGE_BASIS = {"frames": 0, "irreps": 1}      # EQUIGSPR_BASIS_FRAMES / EQUIGSPR_BASIS_IRREPS
