@@ -515,7 +515,9 @@ typedef struct equigspr_attention_tensor {
 /* out = softmax over the allowed keys (scale Q K^T) V.  Key j is allowed for point i of sample b when i < q_lens[b], j < kv_lens[b],
  * key_mask[b][j] != 0 and, if causal, j - kv_lens[b] <= i - q_lens[b] (the last point sees every key).  heads is a multiple of kv_heads:
  * query head h reads key head h / (heads / kv_heads).  1 <= dim <= 128, scale > 0.  Lengths are clamped to [0, nq] / [0, nk]; null = all.
- * Rows without an allowed key, and rows at or behind q_lens[b], give zeros.  Values of keys that are not allowed are never used. */
+ * Rows without an allowed key, and rows at or behind q_lens[b], give zeros.
+ * Values of keys hidden by kv_lens or key_mask are never used; a key that causal hides from some points has weight zero there and must
+ * be finite.  Points and heads lie less than 2^31 / 128 bytes apart. */
 typedef struct equigspr_attention {
     int32_t dtype, batch, nq, nk, heads, kv_heads, dim, causal;
     float   scale;

@@ -38,8 +38,9 @@ def cloud_attention(q, k, v, *, q_lens=None, kv_lens=None, key_mask=None, causal
     ``key_mask`` (bool ``[B, Nk]``): False hides a key.  ``causal``: point ``i`` sees the keys up to ``i + kv_len - q_len``.
     ``scale``: positive, default ``D ** -0.5``.
 
-    A point without a visible key, and a point behind ``q_lens``, gives zeros and takes no gradient; values of hidden keys are never
-    used, whatever they hold, and their gradients are zero.  Differentiable once in q, k and v; bitwise reproducible (no atomics).
+    A point without a visible key, and a point behind ``q_lens``, gives zeros and takes no gradient.  Keys hidden by ``kv_lens`` or
+    ``key_mask`` are never used, whatever they hold, and their gradients are zero; a key that ``causal`` hides from some points only has
+    weight zero there, so its values must be finite.  Differentiable once in q, k and v; bitwise reproducible (no atomics).
     Scores, probabilities' sums and gradients' sums are fp32."""
     need_float(q, "q", ndim=4)
     need_float(k, "k", like=q, ndim=4)

@@ -621,7 +621,7 @@ static int ff_check(const equigspr_gated_feed_forward* d) {
     EQ_CHECK_ARG(d->dtype == EQUIGSPR_F32 || d->dtype == EQUIGSPR_BF16 || d->dtype == EQUIGSPR_F16, EQUIGSPR_EINVAL, "gated_feed_forward: unknown dtype %d", d->dtype);
     EQ_CHECK_ARG(d->activation == kSilu || d->activation == kGelu || d->activation == kRelu, EQUIGSPR_EINVAL, "gated_feed_forward: unknown activation %d", d->activation);
     EQ_CHECK_ARG(d->rows >= 0 && d->width >= 1 && d->hidden >= 1 && d->out >= 1, EQUIGSPR_EINVAL, "gated_feed_forward: bad sizes");
-    EQ_CHECK_ARG(d->rows < (1 << 23) && d->width < (1 << 20) && d->hidden < (1 << 20) && d->out < (1 << 20), EQUIGSPR_ENOTSUP, "gated_feed_forward: sizes beyond the kernels' range");
+    EQ_CHECK_ARG(d->rows <= 65535 * kFfRun && d->width < (1 << 20) && d->hidden < (1 << 20) && d->out < (1 << 20), EQUIGSPR_ENOTSUP, "gated_feed_forward: sizes beyond the kernels' range");
     EQ_CHECK_ARG(d->w_gate && d->w_up && d->w_down && (d->x || !d->rows), EQUIGSPR_EINVAL, "gated_feed_forward: null tensor");
     return 0;
 }

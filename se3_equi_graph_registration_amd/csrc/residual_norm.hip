@@ -157,7 +157,7 @@ __global__ __launch_bounds__(NT) void norm_fwd_kernel(NormArgs<T> a) {
         if (kAhead && r0 + step < s.rows) load(r0 + step);
         if (!kAhead) params();
         if (s.post) {
-            unit_row<kRms>(f, s.eps, s.width, col, sums);
+            unit_row<kRms>(f, row < s.rows ? s.eps : 1.f, s.width, col, sums);
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = fmaf(f[i], post_w[i], post_b[i]);
         }
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(NT) void norm_fwd_kernel(NormArgs<T> a) {
         for (int i = 0; i < 8; ++i) x[i] = fmaf(w[i], f[i], x[i]);
         if (ok && a.y) store8<T>(a.y + at, x, s.width - col);
         if (s.pre) {
-            unit_row<kRms>(x, s.eps, s.width, col, sums);
+            unit_row<kRms>(x, row < s.rows ? s.eps : 1.f, s.width, col, sums);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], pre_w[i], pre_b[i]);
             if (ok) store8<T>(a.u + at, x, s.width - col);
@@ -243,6 +243,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(NormArgs<T> a) {
         for (int64_t r0 = first; r0 < end; r0 += G) {
             const int64_t row = r0 + threadIdx.x / L, at = row * s.width + col;
             const bool ok = row < end && col < s.width;
+            const float eps = row < end ? s.eps : 1.f;      // rows behind the run are zeros: without a spread, eps = 0 would make them NaN in the sums
             float x[8], f[8], gy[8], gu[8], z[8], fr = 1.f;
             if (!kAhead) load(r0);
             row_values<T>(nf, f);
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(NormArgs<T> a) {
             if (kAhead && r0 + G < end) load(r0 + G);
             if (!kAhead) params();
             if (s.post) {
-                fr = unit_row<kRms>(f, s.eps, s.width, col, sums);
+                fr = unit_row<kRms>(f, eps, s.width, col, sums);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) z[i] = fmaf(f[i], post_w[i], post_b[i]);
             } else {
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(NormArgs<T> a) {
             if (s.pre) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] = fmaf(scale[i] * gate[i], z[i], x[i]);
-                const float yr = unit_row<kRms>(x, s.eps, s.width, col, sums);
+                const float yr = unit_row<kRms>(x, eps, s.width, col, sums);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     s_prew[i] = fmaf(gu[i], x[i], s_prew[i]);

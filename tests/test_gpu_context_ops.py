@@ -143,6 +143,27 @@ def test_attention_strides(dtype):
     torch.testing.assert_close(ga, gb.sum(0, keepdim=True), rtol=2 * torch.finfo(dtype).eps, atol=2 * torch.finfo(dtype).eps)
 
 
+@pytest.mark.parametrize("layout", ["far samples", "far points"])
+def test_attention_offsets_beyond_32_bits(layout):
+    """Keys and values whose offsets pass 2^31 values: samples far apart, and a cache with points far apart; forward and backward."""
+    g = torch.Generator().manual_seed(15)
+    b, nk, stride = (2, 70, (2200000000, 64, 64, 1)) if layout == "far samples" else (1, 600, (1, 4000000, 64, 1))
+    buf = torch.empty(2400100000, dtype=torch.bfloat16, device="cuda")
+    k, v = normal(g, b, nk, 1, 64, dtype=torch.bfloat16), normal(g, b, nk, 1, 64, dtype=torch.bfloat16)
+    q, go = normal(g, b, 40, 1, 64, dtype=torch.bfloat16).cuda(), normal(g, b, 40, 1, 64, dtype=torch.bfloat16).cuda()
+    far = []
+    for i, t in enumerate((k, v)):
+        view = buf.as_strided((b, nk, 1, 64), stride, 10000 * i)
+        view.copy_(t)
+        far.append(view)
+
+    def run(kk, vv):
+        a = [t.detach().requires_grad_(True) for t in (q, kk, vv)]
+        out = pkg().cloud_attention(*a)
+        return [out.detach()] + list(torch.autograd.grad(out, a, go))
+    assert all(torch.equal(x, y) for x, y in zip(run(k.cuda(), v.cuda()), run(*far)))
+
+
 @pytest.mark.parametrize("dtype", [torch.float16], ids=["f16"])
 @pytest.mark.parametrize("size", [1e-4, 1e3])
 def test_attention_fp16_gradients_of_any_size(dtype, size):
@@ -327,6 +348,42 @@ def test_residual_norm_without_f_and_with_one_gradient(dtype):
         within({"grad_x": gx, "grad_f": gf}, val, err, f"residual_norm gradient of {which} only")
     none = pkg().residual_norm(xs[:0], fs[:0], ws)
     assert none[0].shape == (0, 40) and float(torch.autograd.grad(none[1].sum(), ws)[0].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("rows,c", [(3, 8), (5, 300), (33, 16)])
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+def test_residual_norm_without_eps(rows, c, kind):
+    """eps = 0, with rows that do not fill a workgroup: the rows that are not there leave no trace in the parameters' gradients."""
+    g = torch.Generator().manual_seed(25)
+    x, f, gu = (normal(g, rows, c, dtype=torch.float32) for _ in range(3))
+    w, v = normal(g, c, dtype=torch.float32), normal(g, c, dtype=torch.float32)
+    dev = [t.cuda().requires_grad_(True) for t in (x, f, w, v)]
+    bias = torch.zeros(c, device="cuda").requires_grad_(True) if kind == "layer" else None
+    y, u = pkg().residual_norm(dev[0], dev[1], dev[2], bias, post_weight=dev[3], kind=kind, eps=0.0)
+    got = dict(zip(("grad_x", "grad_f", "grad_pre_weight", "grad_post_weight"), torch.autograd.grad(u, dev, gu.cuda())), y=y, u=u)
+    val, err = orc.residual_norm(x, f, w, None, v, kind=kind, eps=0.0, grad_u=gu)
+    within(got, val, err, f"residual_norm eps 0 {kind} {(rows, c)}")
+
+
+def test_concurrent_streams_share_nothing():
+    """The same calls on two streams at once, each with its own workspace: what one stream alone gives."""
+    g = torch.Generator().manual_seed(26)
+    q = normal(g, 1, 1, 8, 64, dtype=torch.bfloat16).cuda()
+    caches = [normal(g, 1, 20000, 2, 64, dtype=torch.bfloat16).cuda() for _ in range(2)]
+    x, w = normal(g, 400, 64, dtype=torch.float32).cuda(), [normal(g, *s, dtype=torch.float32, scale=0.1).cuda() for s in ((3000, 64), (3000, 64), (64, 3000))]
+    call = lambda i: (pkg().cloud_attention(q, caches[i], caches[i]), pkg().gated_feed_forward(x * (i + 1), *w))  # noqa: E731
+    want = [call(0), call(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, b in got[i]:
+            assert torch.equal(a, want[i][0]) and torch.equal(b, want[i][1])
 
 
 # ------------------------------------------------------------------------------------------------ streams and graphs
