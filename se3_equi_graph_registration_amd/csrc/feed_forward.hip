@@ -42,6 +42,11 @@ struct FfArgs {
     int act;
 };
 
+__device__ __forceinline__ void floats_of(const Raw8<kF32>& r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = raw_float<kF32>(r, i);
+}
+
 // act(z) and its derivative
 __device__ __forceinline__ void activate(int act, float z, float& a, float& d) {
     if (act == kSilu) {
@@ -96,11 +101,12 @@ struct FfTile {
 #pragma unroll
             for (int u = 0; u < kPer; ++u) {
                 const int id = threadIdx.x + u * NT, r = id / (W / 8), c = id % (W / 8) * 8;
+                const auto cut = [](const E* from, int at, int width) { return NT == 512 ? load8_small<T>(from, at, width) : load8<T>(from, at, width); };
                 if constexpr (kAcross) {
-                    raw[u] = k0 + r < k_end ? load8<T>(o.row(k0 + r) + outer0, c, o.len - outer0) : raw_zero<T>();
+                    raw[u] = k0 + r < k_end ? cut(o.row(k0 + r) + outer0, c, o.len - outer0) : raw_zero<T>();
                 } else {
                     const E* row = outer_row(r, false);
-                    raw[u] = row ? load8<T>(row + k0, c, k_end - k0) : raw_zero<T>();
+                    raw[u] = row ? cut(row + k0, c, k_end - k0) : raw_zero<T>();
                 }
             }
         }
@@ -256,8 +262,20 @@ __global__ __launch_bounds__((FfShapeOf<T, kLarge>::kThreads), 2) void ff_produc
             for (int q = 0; q < 4; ++q)
                 *reinterpret_cast<pf32x4*>(out + (lane & 31) * kOutStride + 32 * j + 8 * q + 4 * half) =
                     (pf32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        // kGrad, small tile: what the epilogue reads from memory is requested for all of this block's steps before the first one needs it
+        // (few workgroups, nothing else hides the latency; the large tile has no registers for it and its own neighbours to hide it)
+        constexpr bool kAll = kEpi == kGrad && !kLarge;
+        Raw8<kF32> pz[kAll ? 32 / kRows : 1], pu[kAll ? 32 / kRows : 1];
+        if constexpr (kAll) {
+#pragma unroll
+            for (int p = 0; p < 32 / kRows; ++p) {
+                const float* src = g.zu + (int64_t)min(m0 + om + 32 * i + p * kRows + lane / kLanes, g.m - 1) * 2 * g.n;
+                pz[p] = left > 0 ? load8<kF32>(src, col, g.n) : raw_zero<kF32>();
+                pu[p] = left > 0 ? load8<kF32>(src + g.n, col, g.n) : raw_zero<kF32>();
+            }
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 1
+#pragma unroll(kAll ? 4 : 1)
         for (int r0 = 0; r0 < 32; r0 += kRows) {
             const int r = r0 + lane / kLanes, row = m0 + om + 32 * i + r;
             float v[8], z[8], u[8];
@@ -286,8 +304,13 @@ __global__ __launch_bounds__((FfShapeOf<T, kLarge>::kThreads), 2) void ff_produc
                 }
             } else if constexpr (kEpi == kGrad) {
                 const int64_t at = (int64_t)row * 2 * g.n + col;
-                load8f<kF32>(g.zu + at, left, z);
-                load8f<kF32>(g.zu + at + g.n, left, u);
+                if constexpr (kAll) {
+                    floats_of(pz[r0 / kRows], z);
+                    floats_of(pu[r0 / kRows], u);
+                } else {
+                    load8f<kF32>(g.zu + at, left, z);
+                    load8f<kF32>(g.zu + at + g.n, left, u);
+                }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float a, d;

@@ -175,6 +175,21 @@ __device__ __forceinline__ Raw8<T> load8(const typename Num<T>::type* row, int c
     return r;
 }
 
+// the same value by value behind the last whole chunk: fewer registers (the large feed-forward tiles have none to spare)
+template <int T>
+__device__ __forceinline__ Raw8<T> load8_small(const typename Num<T>::type* row, int col, int width) {
+    Raw8<T> r;
+    if (col + 8 <= width) return load8<T>(row + col, 0, 8);
+    r = raw_zero<T>();
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (col + i < width) {
+            if constexpr (T == kF32) r.v[i >> 2][i & 3] = row[col + i];
+            else r.v[i] = __builtin_bit_cast(short, row[col + i]);
+        }
+    return r;
+}
+
 // A tile of rows of W 16-bit values in LDS.  The rows' stride is padded so that the 16 rows of a ds_read_b128 group start in 16 different
 // bank quads; the four rows of a transposed read then overlap two-fold, which costs a cycle.  (An XOR swizzle has neither conflict but an
 // address register per k-step: in the kernels' keys' gradients at W = 128 that was the difference between one and two waves per SIMD.)
