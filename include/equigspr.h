@@ -4,7 +4,7 @@
  * libequigspr.so (built from the .hip files in se3_equi_graph_registration_amd/csrc for gfx950) exports
  * exactly the entry points below.  Plain pointers and sizes only: no torch types, no C++
  * types.  Every pointer is a DEVICE pointer unless it says "host".  All floating point is
- * fp32; all functions enqueue on `stream` (a hipStream_t passed as void*) and never
+ * fp32 (the context operators also take bf16 and fp16); all functions enqueue on `stream` (a hipStream_t passed as void*) and never
  * synchronise the host, never allocate (hipGraph-capturable: callers own every buffer and
  * size the workspaces with the *_size() helpers).
  *

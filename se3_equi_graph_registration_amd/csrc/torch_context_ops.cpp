@@ -316,7 +316,7 @@ std::tuple<at::Tensor, at::Tensor> residual_norm(const at::Tensor& x, const OptT
     for (const auto* t : {&pre_w, &pre_b, &post_w, &post_b, &scale})
         TORCH_CHECK(!t->has_value() || ((*t)->is_cuda() && (*t)->device() == x.device() && (*t)->scalar_type() == at::kFloat && (*t)->is_contiguous() && (*t)->numel() == width),
                     "equigspr::residual_norm: weights, biases and scale must be float32 [width] on the inputs' device");
-    TORCH_CHECK(gate_rows >= 1 && (!gate.has_value() || (rows % gate_rows == 0 && gate->numel() == rows / gate_rows * width)), "equigspr::residual_norm: the gate does not fit x");
+    TORCH_CHECK(gate_rows >= 1 && (!gate.has_value() || rows == 0 || (rows % gate_rows == 0 && gate->numel() == rows / gate_rows * width)), "equigspr::residual_norm: the gate does not fit x");
     variable_list out;
     if (training({x, value(f), value(pre_w), value(pre_b), value(post_w), value(post_b), value(gate), value(scale)})) {
         auto some = ResidualNormFn::apply(x, f, pre_w, pre_b, post_w, post_b, gate, scale, rms, eps, factor, gate_rows);

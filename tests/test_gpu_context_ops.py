@@ -365,6 +365,17 @@ def test_residual_norm_without_eps(rows, c, kind):
     within(got, val, err, f"residual_norm eps 0 {kind} {(rows, c)}")
 
 
+@pytest.mark.parametrize("gate", ["sample", "all", "one"])
+def test_residual_norm_of_nothing(gate):
+    """Clouds without points: empty outputs, parameter and gate gradients of zeros."""
+    x = torch.zeros(2, 0, 16, device="cuda").requires_grad_(True)
+    w = torch.ones(16, device="cuda").requires_grad_(True)
+    gt = torch.ones({"sample": (2, 16), "all": (2, 0, 16), "one": (16,)}[gate], device="cuda").requires_grad_(True)
+    y, u = pkg().residual_norm(x, x, w, gate=gt)
+    assert y.shape == u.shape == (2, 0, 16)
+    assert all(float(t.abs().sum()) == 0.0 for t in torch.autograd.grad(y.sum() + u.sum(), [x, w, gt]))
+
+
 def test_concurrent_streams_share_nothing():
     """The same calls on two streams at once, each with its own workspace: what one stream alone gives."""
     g = torch.Generator().manual_seed(26)
