@@ -67,19 +67,22 @@ struct RowSums {
     }
 };
 
-template <int T>
+// kEven: width % 8 == 0, no thread's columns are cut (the code for cut ones spills the kernels' scalar registers)
+template <int T, bool kEven>
 __device__ __forceinline__ Raw8<T> load_row(const typename Num<T>::type* row, int width, int col) {
-    return row && col < width ? load8<T>(row, col, width) : raw_zero<T>();
+    if constexpr (kEven) return row && col < width ? load8<T>(row + col, 0, 8) : raw_zero<T>();
+    else return row && col < width ? load8_small<T>(row, col, width) : raw_zero<T>();
 }
 template <int T>
 __device__ __forceinline__ void row_values(const Raw8<T>& r, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = raw_float<T>(r, i);
 }
+template <bool kEven>
 __device__ __forceinline__ void load_columns(const float* p, int width, int col, float otherwise, float (&w)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = otherwise;
-    if (p && col < width) row_values<kF32>(load8<kF32>(p, col, width), w);
+    if (p && col < width) row_values<kF32>(load_row<kF32, kEven>(p, width, col), w);
 }
 
 // v -> its unit row in place (columns behind the width become zero); returns 1 / spread
@@ -122,7 +125,7 @@ __device__ __forceinline__ void unit_row_grad(float (&g)[8], const float (&n)[8]
 
 // The parameters of a thread's columns stay in registers while it walks its rows, and the next row is loaded under this row's arithmetic;
 // the widest rows (1024 threads, 128 registers each) have no room for either.
-template <int T, int L, int NT, bool kRms>
+template <int T, int L, int NT, bool kRms, bool kEven>
 __global__ __launch_bounds__(NT) void norm_fwd_kernel(NormArgs<T> a) {
     constexpr bool kAhead = NT < 1024;
     const NormShape& s = a.s;
@@ -132,18 +135,18 @@ __global__ __launch_bounds__(NT) void norm_fwd_kernel(NormArgs<T> a) {
     const int64_t step = (int64_t)gridDim.x * (NT / L), first = (int64_t)blockIdx.x * (NT / L);
     float post_w[8], post_b[8], pre_w[8], pre_b[8], scale[8];
     auto params = [&] {
-        load_columns(s.post_w, s.width, col, 1.f, post_w);
-        load_columns(s.post_b, s.width, col, 0.f, post_b);
-        load_columns(s.pre_w, s.width, col, 1.f, pre_w);
-        load_columns(s.pre_b, s.width, col, 0.f, pre_b);
-        load_columns(s.scale, s.width, col, s.factor, scale);
+        load_columns<kEven>(s.post_w, s.width, col, 1.f, post_w);
+        load_columns<kEven>(s.post_b, s.width, col, 0.f, post_b);
+        load_columns<kEven>(s.pre_w, s.width, col, 1.f, pre_w);
+        load_columns<kEven>(s.pre_b, s.width, col, 0.f, pre_b);
+        load_columns<kEven>(s.scale, s.width, col, s.factor, scale);
     };
     Raw8<T> nx, nf;
     auto load = [&](int64_t r0) {
         const int64_t row = r0 + threadIdx.x / L;
         const bool ok = row < s.rows;
-        nx = load_row<T>(ok ? a.x + row * s.width : nullptr, s.width, col);
-        nf = load_row<T>(ok && a.f ? a.f + row * s.width : nullptr, s.width, col);
+        nx = load_row<T, kEven>(ok ? a.x + row * s.width : nullptr, s.width, col);
+        nf = load_row<T, kEven>(ok && a.f ? a.f + row * s.width : nullptr, s.width, col);
     };
     if (kAhead) {
         params();
@@ -167,18 +170,18 @@ __global__ __launch_bounds__(NT) void norm_fwd_kernel(NormArgs<T> a) {
         for (int i = 0; i < 8; ++i) w[i] = scale[i];
         if (a.gate) {
             float g[8];
-            row_values<T>(load_row<T>(row < s.rows ? a.gate + row / s.gate_rows * s.width : nullptr, s.width, col), g);
+            row_values<T>(load_row<T, kEven>(row < s.rows ? a.gate + row / s.gate_rows * s.width : nullptr, s.width, col), g);
 #pragma unroll
             for (int i = 0; i < 8; ++i) w[i] *= g[i];
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = fmaf(w[i], f[i], x[i]);
-        if (ok && a.y) store8<T>(a.y + at, x, s.width - col);
+        if (ok && a.y) store8<T>(a.y + at, x, kEven ? 8 : s.width - col);
         if (s.pre) {
             unit_row<kRms>(x, row < s.rows ? s.eps : 1.f, s.width, col, sums);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], pre_w[i], pre_b[i]);
-            if (ok) store8<T>(a.u + at, x, s.width - col);
+            if (ok) store8<T>(a.u + at, x, kEven ? 8 : s.width - col);
         }
     }
 }
@@ -205,7 +208,7 @@ __device__ __forceinline__ void group_columns(const float (&acc)[8], float* lds,
     }
 }
 
-template <int T, int L, int NT, bool kRms>
+template <int T, int L, int NT, bool kRms, bool kEven>
 __global__ __launch_bounds__(NT) void norm_bwd_kernel(NormArgs<T> a) {
     constexpr int G = NT / L;
     constexpr bool kAhead = NT < 1024;
@@ -219,10 +222,10 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(NormArgs<T> a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) { s_prew[i] = s_preb[i] = s_postw[i] = s_postb[i] = s_scale[i] = 0.f; gate[i] = 1.f; }
     auto params = [&] {
-        load_columns(s.post_w, s.width, col, 1.f, post_w);
-        load_columns(s.post_b, s.width, col, 0.f, post_b);
-        load_columns(s.pre_w, s.width, col, 1.f, pre_w);
-        load_columns(s.scale, s.width, col, s.factor, scale);
+        load_columns<kEven>(s.post_w, s.width, col, 1.f, post_w);
+        load_columns<kEven>(s.post_b, s.width, col, 0.f, post_b);
+        load_columns<kEven>(s.pre_w, s.width, col, 1.f, pre_w);
+        load_columns<kEven>(s.scale, s.width, col, s.factor, scale);
     };
     if (kAhead) params();
     for (int64_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
@@ -231,15 +234,15 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(NormArgs<T> a) {
         float s_z[8];                         // sum of grad_y_total * z: the gate's gradient up to the scale, the scale's up to the gate
 #pragma unroll
         for (int i = 0; i < 8; ++i) s_z[i] = 0.f;
-        if (a.gate) row_values<T>(load_row<T>(a.gate + gate_row * s.width, s.width, col), gate);
+        if (a.gate) row_values<T>(load_row<T, kEven>(a.gate + gate_row * s.width, s.width, col), gate);
         Raw8<T> nx, nf, ngy, ngu;
         auto load = [&](int64_t r0) {
             const int64_t row = r0 + threadIdx.x / L, at = row * s.width;
             const bool ok = row < end;
-            nf = load_row<T>(ok && a.f ? a.f + at : nullptr, s.width, col);
-            nx = load_row<T>(ok ? a.x + at : nullptr, s.width, col);
-            ngu = load_row<T>(ok && a.gu ? a.gu + at : nullptr, s.width, col);
-            ngy = load_row<T>(ok && a.gy ? a.gy + at : nullptr, s.width, col);
+            nf = load_row<T, kEven>(ok && a.f ? a.f + at : nullptr, s.width, col);
+            nx = load_row<T, kEven>(ok ? a.x + at : nullptr, s.width, col);
+            ngu = load_row<T, kEven>(ok && a.gu ? a.gu + at : nullptr, s.width, col);
+            ngy = load_row<T, kEven>(ok && a.gy ? a.gy + at : nullptr, s.width, col);
         };
         if (kAhead) load(first);
         for (int64_t r0 = first; r0 < end; r0 += G) {
@@ -276,7 +279,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(NormArgs<T> a) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) gy[i] += gu[i];
             }
-            if (ok && a.gx) store8<T>(a.gx + at, gy, s.width - col);
+            if (ok && a.gx) store8<T>(a.gx + at, gy, kEven ? 8 : s.width - col);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 s_z[i] = fmaf(gy[i], z[i], s_z[i]);
@@ -291,7 +294,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(NormArgs<T> a) {
                 }
                 if (a.gf) unit_row_grad<kRms>(gy, f, fr, s.width, col, sums);
             }
-            if (ok && a.gf) store8<T>(a.gf + at, gy, s.width - col);
+            if (ok && a.gf) store8<T>(a.gf + at, gy, kEven ? 8 : s.width - col);
         }
         if (!kAhead) params();
 #pragma unroll
@@ -363,12 +366,17 @@ static NormPlan norm_plan(const NormShape& s, bool gated) {
 template <int T>
 static int norm_run(const NormArgs<T>& a, bool backward, int blocks, hipStream_t st) {
     const int w = a.s.width;
-#define EQ_NORM(L, NT)                                                                              \
-    do {                                                                                            \
-        if (backward && a.s.rms) norm_bwd_kernel<T, L, NT, true><<<blocks, NT, 0, st>>>(a);         \
-        else if (backward) norm_bwd_kernel<T, L, NT, false><<<blocks, NT, 0, st>>>(a);              \
-        else if (a.s.rms) norm_fwd_kernel<T, L, NT, true><<<blocks, NT, 0, st>>>(a);                \
-        else norm_fwd_kernel<T, L, NT, false><<<blocks, NT, 0, st>>>(a);                            \
+#define EQ_NORM_EVEN(L, NT, EVEN)                                                                       \
+    do {                                                                                                \
+        if (backward && a.s.rms) norm_bwd_kernel<T, L, NT, true, EVEN><<<blocks, NT, 0, st>>>(a);       \
+        else if (backward) norm_bwd_kernel<T, L, NT, false, EVEN><<<blocks, NT, 0, st>>>(a);            \
+        else if (a.s.rms) norm_fwd_kernel<T, L, NT, true, EVEN><<<blocks, NT, 0, st>>>(a);              \
+        else norm_fwd_kernel<T, L, NT, false, EVEN><<<blocks, NT, 0, st>>>(a);                          \
+    } while (0)
+#define EQ_NORM(L, NT)                       \
+    do {                                     \
+        if (w % 8 == 0) EQ_NORM_EVEN(L, NT, true); \
+        else EQ_NORM_EVEN(L, NT, false);     \
     } while (0)
     if (w <= 64) EQ_NORM(8, 256);
     else if (w <= 512) EQ_NORM(64, 256);
@@ -376,6 +384,7 @@ static int norm_run(const NormArgs<T>& a, bool backward, int blocks, hipStream_t
     else if (w <= 4096) EQ_NORM(512, 512);
     else EQ_NORM(1024, 1024);
 #undef EQ_NORM
+#undef EQ_NORM_EVEN
     EQ_CHECK_LAUNCH(backward ? "residual_norm_backward" : "residual_norm_forward");
     return 0;
 }

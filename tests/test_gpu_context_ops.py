@@ -279,7 +279,7 @@ def test_feed_forward_empty_partial_and_unaligned(dtype):
 # ------------------------------------------------------------------------------------------------ residual norm
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("kind", ["layer", "rms"])
-@pytest.mark.parametrize("b,n,c", [(1, 1, 1), (2, 3, 7), (2, 100, 32), (3, 17, 33), (2, 9, 64), (1, 40, 65), (2, 30, 512), (2, 7, 1000), (1, 5, 2048), (1, 3, 3000),
+@pytest.mark.parametrize("b,n,c", [(1, 1, 1), (2, 3, 7), (2, 100, 32), (3, 17, 33), (2, 9, 64), (1, 40, 65), (2, 30, 512), (2, 7, 1000), (1, 5, 2048), (1, 3, 3000), (2, 6, 1001), (1, 3, 4099),
                                    (1, 2, 8192)])
 def test_residual_norm_shapes(dtype, kind, b, n, c):
     residual_norm_case(21, dtype, kind, b, n, c)
