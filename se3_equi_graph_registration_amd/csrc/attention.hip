@@ -161,7 +161,11 @@ __global__ __launch_bounds__(NW * 64, W == 128 && T == kF32 ? 1 : 2) void attn_f
                 for (int j = 0; j < 8; ++j) x[j] = sc[kb][8 * t + j];
                 const Op8<T> p = pack8<T>(x);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) mma<T>(acc[d], tile_cols<T, W, KT>(tile_v, kb * 32 + 16 * t, d * 32, lane), p);
+                for (int d = 0; d < DB; ++d) {
+                    const Op8<T> v = tile_cols<T, W, KT>(tile_v, kb * 32 + 16 * t, d * 32, lane);
+                    if constexpr (attn_two_planes<T, KS>()) mma<T>(acc[d], v, pack8_rest<T>(x));
+                    mma<T>(acc[d], v, p);
+                }
             }
     }
     if (row >= rows) return;

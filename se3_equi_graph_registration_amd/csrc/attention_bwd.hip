@@ -200,7 +200,11 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_ker
                     x[j] = exp2_fast(fmaf(sc[8 * t + j], s.scale_log2, -lse)) * (dp[8 * t + j] - delta) * factor;
                 const Op8<T> ds = pack8<T>(x);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) mma<T>(acc[d], tile_cols<T, W, KT>(tile_k, kb * 32 + 16 * t, d * 32, lane), ds);
+                for (int d = 0; d < DB; ++d) {
+                    const Op8<T> kt = tile_cols<T, W, KT>(tile_k, kb * 32 + 16 * t, d * 32, lane);
+                    if constexpr (attn_two_planes<T, KS>()) mma<T>(acc[d], kt, pack8_rest<T>(x));
+                    mma<T>(acc[d], kt, ds);
+                }
             }
         }
     }
@@ -341,8 +345,13 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dkv_ke
                 const Op8<T> p = pack8<T>(x), ds = pack8<T>(y);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    mma<T>(acc_v[d], tile_cols<T, W, RT>(tile_g, rb * 32 + 16 * t, d * 32, lane), p);
-                    mma<T>(acc_k[d], tile_cols<T, W, RT>(tile_q, rb * 32 + 16 * t, d * 32, lane), ds);
+                    const Op8<T> gt = tile_cols<T, W, RT>(tile_g, rb * 32 + 16 * t, d * 32, lane), qt = tile_cols<T, W, RT>(tile_q, rb * 32 + 16 * t, d * 32, lane);
+                    if constexpr (attn_two_planes<T, KS>()) {
+                        mma<T>(acc_v[d], gt, pack8_rest<T>(x));
+                        mma<T>(acc_k[d], qt, pack8_rest<T>(y));
+                    }
+                    mma<T>(acc_v[d], gt, p);
+                    mma<T>(acc_k[d], qt, ds);
                 }
             }
         }

@@ -126,6 +126,10 @@ __device__ __forceinline__ AttnUnit attn_unit(int heads, int units) {
     return {32 * group + r % n, r / n};
 }
 
+// 16-bit heads of up to 16 dims: P and dS enter their products in two planes.  Their rounding hardly averages out there (gradients of q 1.6
+// times as far off as the plain form's, 1.4 for wider heads), and the second product is one matrix instruction.
+template <int T, int KS> constexpr bool attn_two_planes() { return T != kF32 && KS == 1; }
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 constexpr int kAttnMaxDim = 128;

@@ -95,6 +95,15 @@ __device__ __forceinline__ Op8<T> pack8(const float (&x)[8]) {
     return r;
 }
 
+// what the rounding of pack8 dropped, as an operand of the same 16-bit type
+template <int T>
+__device__ __forceinline__ Op8<T> pack8_rest(const float (&x)[8]) {
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i] - (float)(typename Num<T>::type)x[i];
+    return pack8<T>(r);
+}
+
 template <int T>
 __device__ __forceinline__ Op8<T> planes_of(const Raw8<T>& raw) {
     if constexpr (T == kF32) {
