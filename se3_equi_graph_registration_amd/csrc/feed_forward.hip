@@ -244,10 +244,29 @@ __global__ __launch_bounds__((FfShapeOf<T, kLarge>::kThreads), 2) void ff_produc
             __syncthreads();
             if (k0 + BK < k_end) load(k0 + BK);
             fetch(0, 0, 0);
+            if constexpr (T == kF32) {
+                // The twelve products of a k tile in an accumulator of their own, added by the vector ALU: the matrix pipe does not round
+                // to nearest when it adds to a large accumulator, and what that leaves adds up in sums over rows (biases' gradients).
+                static_assert(KS == 2, "both steps' operands are held at once");
+                fetch(0, 1, 1);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                if (ks + 1 < KS) fetch(0, ks + 1, (ks + 1) & 1);
-                products(ks & 1);
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        pf32x16 t;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) t[r] = 0.f;
+#pragma unroll
+                        for (int ks = 0; ks < KS; ++ks) mma<T>(t, pb[ks][j], pa[ks][i]);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[i][j][r] += t[r];
+                    }
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    if (ks + 1 < KS) fetch(0, ks + 1, (ks + 1) & 1);
+                    products(ks & 1);
+                }
             }
         }
     }
