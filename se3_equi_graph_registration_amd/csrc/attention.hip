@@ -4,7 +4,8 @@
 // rows (attention_device.h): the products are formed transposed, S^T = K Q^T (C tile: lane = row, registers = keys), so the softmax of
 // a row is a loop over one lane's registers plus one exchange with lane ^ 32, and P^T is the B operand of O^T = V^T P^T as it stands
 // (tile_cols reads V in the matching key order).  Statistics, P and O are fp32; P is rounded to the inputs' 16-bit type for the second
-// product (relative 2^-9 / 2^-12 of each probability, averaged over the keys; fp32 keeps all three planes).
+// product (at most 2^-8 / 2^-11 of each probability, averaged over the keys; heads of up to 16 dims take a second plane with what that
+// drops, fp32 keeps all three).
 // Few rows against many keys: the key axis is split over workgroups, each writes its normalised part and its log-sum, and
 // attn_join_kernel joins them in split order (no atomics: results do not depend on timing).
 // Bound: the vector ALU up to heads of 64 (160 instructions of softmax per 16 products of a 64-key tile), the matrix pipe at 128.  Measured,

@@ -4,8 +4,9 @@
 // attn_dkv_kernel owns 32 keys per wave and walks the packed rows -- all query heads of the group, so the gradients of shared keys need
 // no atomics and do not depend on timing.  In each, the score tile is formed with the owned index in the lane, which makes P and dS the
 // B operands of the products that follow as they stand (see attention.hip); the other operand is the staged tile read transposed.
-// P and dS are rounded to the inputs' 16-bit type for those products, everything else is fp32; the forward leaves what the output's
-// rounding dropped in a second plane for delta, whose error every dS of the row would share.
+// P and dS are rounded to the inputs' 16-bit type for those products (heads of up to 16 dims take a second plane with what that
+// drops), everything else is fp32; the forward leaves what the output's rounding dropped in a second plane for delta, whose error every
+// dS of the row would share.
 // Bound: as the forward, and the registers -- the accumulators of wide heads leave two waves per SIMD.  Measured, bf16: 8 x 2048^2 x 8 heads
 // of 64 340 us (505 TFLOP/s of the five products that the mathematics needs), 8192^2 x 16 / 4 heads of 128 2.0 ms (680), causal 1.14 ms.
 // fp16: dS is about 1/keys of the output gradient and would sink below fp16's range, so it is held as 2^E dS, with E from the largest

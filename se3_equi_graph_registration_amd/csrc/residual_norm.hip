@@ -4,8 +4,8 @@
 // One pass over memory: a row stays in the registers of L threads (8, 64, 256, 512 or 1024) from its loads to its stores, so the forward
 // moves x, f, y, u once and the backward x, f, grad_y, grad_u, grad_x, grad_f once -- the backward recomputes both norms from x and f
 // instead of reading anything the forward kept.  Bound: HBM forward
-// (32768 x 2048 bf16: 111 us, 4.8 TB/s); backward the registers of its column sums, which leave two workgroups per compute unit (266 us,
-// 3.0 TB/s).  All sums are fp32, the spread is taken about the mean (two sums), y
+// (32768 x 2048 bf16: 111 us, 4.8 TB/s); backward the registers of its column sums, which leave two workgroups per compute unit (250 us,
+// 3.2 TB/s).  All sums are fp32, the spread is taken about the mean (two sums), y
 // enters the second norm before its rounding to the output type.
 // Parameter gradients are column sums: every workgroup sums its rows in registers, norm_columns_kernel adds the workgroups' partial
 // rows in order.  The gate's gradient is a sum over the rows that share a gate row: a workgroup takes whole runs of them.
