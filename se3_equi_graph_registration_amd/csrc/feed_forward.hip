@@ -58,9 +58,9 @@ __device__ __forceinline__ void activate(int act, float z, float& a, float& d) {
         const float c = 0.5f * (1.f + erff(z * 0.70710678118654752f));
         a = z * c;
         d = fmaf(z * 0.39894228040143268f, __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z), c);
-    } else {
-        a = fmaxf(z, 0.f);
-        d = z > 0.f ? 1.f : 0.f;
+    } else {                                      // NaN stays NaN in both
+        a = z <= 0.f ? 0.f : z;
+        d = z > 0.f ? 1.f : z <= 0.f ? 0.f : z;
     }
 }
 

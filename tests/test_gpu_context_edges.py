@@ -1,0 +1,32 @@
+"""The context operators where the ordinary cases do not lead: non-finite values that are seen, points without a key, gradients of very
+different sizes, sizes beyond 32 bits, forward-mode derivatives, more heads, rows and units than one trip of a loop takes.  Against the fp64
+definitions (oracle/context_oracle.py) or the operators' own promises."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from oracle import context_oracle as orc  # noqa: E402
+from tests.test_gpu_context_ops import IDS, TYPES, attention_case, normal, pkg, residual_norm_case, within  # noqa: E402
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("activation", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("where", ["w_gate", "b_gate"])
+@pytest.mark.parametrize("rows", [5, 200])
+def test_feed_forward_nan_in_the_gate_is_seen(dtype, activation, where, rows):
+    """One hidden unit whose gate is NaN: every output and every gradient that it enters is NaN, the other units' gradients are finite.
+    Few rows and tiles."""
+    g = torch.Generator().manual_seed(41)
+    t = {"x": normal(g, rows, 24, dtype=dtype), "w_gate": normal(g, 40, 24, dtype=dtype, scale=0.2), "w_up": normal(g, 40, 24, dtype=dtype, scale=0.2),
+         "w_down": normal(g, 20, 40, dtype=dtype, scale=0.2), "b_gate": normal(g, 40, dtype=dtype)}
+    (t[where][7, 3:4] if where == "w_gate" else t[where][7:8]).fill_(float("nan"))
+    dev = {n: v.cuda().requires_grad_(True) for n, v in t.items()}
+    y = pkg().gated_feed_forward(**dev, activation=activation)
+    assert y.isnan().all()
+    got = dict(zip(dev, torch.autograd.grad(y, list(dev.values()), normal(g, rows, 20, dtype=dtype).cuda())))
+    assert got["x"].isnan().all()
+    others = torch.arange(40, device="cuda") != 7
+    for n in ("w_gate", "w_up", "b_gate"):
+        assert got[n][7].isnan().all() and got[n][others].isfinite().all(), n
+    assert got["w_down"][:, 7].isnan().all() and got["w_down"][:, others].isfinite().all()
