@@ -40,7 +40,7 @@ def cloud_attention(q, k, v, *, q_lens=None, kv_lens=None, key_mask=None, causal
 
     A point without a visible key, and a point behind ``q_lens``, gives zeros and takes no gradient.  Keys hidden by ``kv_lens`` or
     ``key_mask`` are never used, whatever they hold, and their gradients are zero; a key that ``causal`` hides from some points only has
-    weight zero there, so its values must be finite.  Differentiable once in q, k and v; bitwise reproducible (no atomics).
+    weight zero there, so its values must be finite.  Differentiable once in q, k and v (reverse mode; tangents are refused); bitwise reproducible (no atomics).
     Scores, probabilities' sums and gradients' sums are fp32."""
     need_float(q, "q", ndim=4)
     need_float(k, "k", like=q, ndim=4)

@@ -56,8 +56,11 @@ bool grad_lives_on_other_stream(const at::Tensor& t) {
     if (hipStreamIsCapturing(other.stream(), &status) != hipSuccess) { (void)hipGetLastError(); return true; }
     return status != hipStreamCaptureStatusActive;
 }
-// true if one of the inputs wants a gradient; refuses a capture that would end the process
+// true if one of the inputs wants a gradient; refuses a capture that would end the process, and tangents, which the output would lose
 bool training(std::initializer_list<at::Tensor> inputs) {
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        for (const auto& t : inputs)
+            TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "equigspr: the context operators have no forward-mode derivative");
     if (!at::GradMode::is_enabled()) return false;
     bool any = false;
     at::Tensor one;

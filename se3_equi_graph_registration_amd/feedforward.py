@@ -18,7 +18,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
     (exact) or "relu".  Products accumulate in fp32; the hidden layer is held in the inputs' dtype between the two products, as are the
     projections' gradients in the backward: in float16 they must stay within that type's range.  The backward keeps both projections in
     float32.  Up to 8 388 480 rows a call.  Differentiable once in every
-    tensor; bitwise reproducible (no atomics)."""
+    tensor (reverse mode; tangents are refused); bitwise reproducible (no atomics)."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"gated_feed_forward: activation {activation!r}, expected one of {sorted(ACTIVATIONS)}")
     need_float(x, "x")

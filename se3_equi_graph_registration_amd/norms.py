@@ -20,7 +20,8 @@ def residual_norm(x, f, pre_weight=None, pre_bias=None, *, post_weight=None, pos
     ``x``, ``f [..., C]``: float32, bfloat16 or float16, alike, ``1 <= C <= 8192`` (copied if not contiguous).  ``kind``: "layer" (mean and
     spread) or "rms" (spread about zero, no mean).  ``gate`` (dtype of x): ``[C]``, one row per sample ``[B, C]`` for ``x [B, N, C]``, or the
     shape of ``x``.  ``scale``: a float or a tensor ``[C]``.  Weights, biases and a tensor scale are used in float32 (converted if not).
-    Sums are fp32, the second norm takes ``y`` before its rounding.  Differentiable once in every tensor; bitwise reproducible."""
+    Sums are fp32, the second norm takes ``y`` before its rounding.  Differentiable once in every tensor (reverse mode;
+    tangents are refused); bitwise reproducible."""
     if kind not in KINDS:
         raise ValueError(f"residual_norm: kind {kind!r}, expected 'layer' or 'rms'")
     need_float(x, "x")

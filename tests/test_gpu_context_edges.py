@@ -30,3 +30,22 @@ def test_feed_forward_nan_in_the_gate_is_seen(dtype, activation, where, rows):
     for n in ("w_gate", "w_up", "b_gate"):
         assert got[n][7].isnan().all() and got[n][others].isfinite().all(), n
     assert got["w_down"][:, 7].isnan().all() and got["w_down"][:, others].isfinite().all()
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent on any input would be lost (the output would carry none: a derivative of zero), so the operators raise."""
+    from torch.autograd import forward_ad
+    ones = lambda *s: torch.ones(*s, device="cuda")  # noqa: E731
+    att, ff, rn = pkg().cloud_attention, pkg().gated_feed_forward, pkg().residual_norm
+    q, x, w, wd, c = ones(1, 4, 2, 8), ones(3, 8), ones(6, 8), ones(8, 6), ones(8)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for bad in (lambda: att(dual(q), q, q), lambda: att(q, q, dual(q)), lambda: ff(dual(x), w, w, wd), lambda: ff(x, w, w, dual(wd)),
+                    lambda: ff(x, w, w, wd, b_down=dual(c)), lambda: rn(dual(x), x, c), lambda: rn(x, x, dual(c)), lambda: rn(x, x, gate=dual(c)),
+                    lambda: att(dual(q.clone().requires_grad_(True)), q, q)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                bad()
+        with torch.no_grad():                                              # forward mode does not ask for gradients to be enabled
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                att(dual(q), q, q)
+        att(q, q, q)                                                       # no tangent: nothing is lost
