@@ -32,6 +32,8 @@ int dtype_code(const at::Tensor& t) {
         default: TORCH_CHECK(false, "equigspr: expected float32, bfloat16 or float16, got ", t.scalar_type());
     }
 }
+// sizes that the C entries count in 32 bits
+bool counted(int64_t n) { return n < (1ll << 31); }
 // on the GPU, of one type and device with `like`, and (dense) contiguous
 void need(const at::Tensor& t, const at::Tensor& like, const char* name, bool dense) {
     if (!t.defined()) return;
@@ -102,6 +104,7 @@ equigspr_attention describe(const at::Tensor& q, const at::Tensor& k, const at::
                             bool causal, double scale) {
     equigspr_attention d = {};
     d.dtype = dtype_code(q);
+    for (int i = 0; i < 3; ++i) TORCH_CHECK(counted(q.size(i)) && counted(k.size(i)), "equigspr::cloud_attention: sizes out of range");
     d.batch = (int32_t)q.size(0); d.nq = (int32_t)q.size(1); d.nk = (int32_t)k.size(1);
     d.heads = (int32_t)q.size(2); d.kv_heads = (int32_t)k.size(2); d.dim = (int32_t)q.size(3);
     d.causal = causal;
@@ -179,7 +182,7 @@ equigspr_gated_feed_forward describe(const at::Tensor& x, const at::Tensor& wg, 
     equigspr_gated_feed_forward d = {};
     d.dtype = dtype_code(x);
     d.activation = (int32_t)act;
-    TORCH_CHECK(x.size(0) < (1ll << 31) && x.size(1) < (1ll << 31) && wg.size(0) < (1ll << 31) && wd.size(0) < (1ll << 31), "equigspr::gated_feed_forward: sizes out of range");
+    TORCH_CHECK(counted(x.size(0)) && counted(x.size(1)) && counted(wg.size(0)) && counted(wd.size(0)), "equigspr::gated_feed_forward: sizes out of range");
     d.rows = (int32_t)x.size(0); d.width = (int32_t)x.size(1); d.hidden = (int32_t)wg.size(0); d.out = (int32_t)wd.size(0);
     d.x = cptr(x); d.w_gate = cptr(wg); d.w_up = cptr(wu); d.w_down = cptr(wd);
     d.b_gate = cptr(bg); d.b_up = cptr(bu); d.b_down = cptr(bd);
@@ -251,6 +254,7 @@ equigspr_residual_norm describe(const variable_list& t, const NormRest& r) {    
     equigspr_residual_norm d = {};
     const at::Tensor& x = t[0];
     d.dtype = dtype_code(x);
+    TORCH_CHECK(counted(x.size(-1)), "equigspr::residual_norm: width out of range");
     d.width = (int32_t)x.size(-1);
     d.rms = r.rms;
     d.rows = x.numel() / x.size(-1);

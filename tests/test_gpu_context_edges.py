@@ -49,3 +49,16 @@ def test_forward_mode_derivatives_are_refused():
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 att(dual(q), q, q)
         att(q, q, q)                                                       # no tangent: nothing is lost
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Broadcast views with more points than 32 bits count: refused, not taken modulo 2^32."""
+    one = torch.ones(1, 1, 1, 1, dtype=torch.bfloat16, device="cuda")
+    many = one.expand(1, 2 ** 32 + 5, 1, 1)
+    with pytest.raises(RuntimeError, match="range"):
+        pkg().cloud_attention(one, many, many)
+    with pytest.raises(RuntimeError, match="range"):
+        pkg().cloud_attention(many, one, one)
+    row = torch.empty(1, 2 ** 32 + 8, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="range"):
+        torch.ops.equigspr.residual_norm(row, row, None, None, None, None, None, None, False, 1e-5, 1.0, 1)
