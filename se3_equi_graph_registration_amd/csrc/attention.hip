@@ -21,7 +21,7 @@ struct AttnFwd {
     AttnTensor<T> q, k, v;
     typename Num<T>::type* out;               // [batch, nq, heads, dim] contiguous
     typename Num<T>::type* out_low;           // 16-bit types, for the backward: what out's rounding dropped, or null
-    float* lse;                               // [batch, kv_heads, nq * group] base-2 log-sum of the scaled scores, +inf for a row without keys
+    float* lse;                               // [batch, kv_heads, nq * group] base-2 log-sum of the scaled scores, +inf for a row without keys, NaN for a NaN sum
     int row_tiles, splits, split_keys;
     float* part_o;                            // [splits][batch * kv_heads][nq * group][dim]
     float* part_l;                            // [splits][batch * kv_heads][nq * group], -inf for a part without keys
@@ -171,13 +171,14 @@ __global__ __launch_bounds__(NW * 64, W == 128 && T == kF32 ? 1 : 2) void attn_f
     }
     if (row >= rows) return;
     l += __shfl_xor(l, 32);
-    const bool exists = row < rows_valid, some = exists && l > 0.f;
+    const bool exists = row < rows_valid;
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a NaN sum stays NaN, an empty row becomes zero
-    const float lse = some ? fmaf(m, s.scale_log2, log2f(l) - kShift) : INFINITY;
+    // a row without keys: +inf (its probabilities are zero); a NaN sum stays NaN, so that the backward's probabilities are NaN for all its keys
+    const float lse = !exists || l == 0.f ? INFINITY : fmaf(m, s.scale_log2, log2f(l) - kShift);
     const int64_t at = (int64_t)bh * rows + row;
     if (a.splits > 1) {
         const int64_t pat = ((int64_t)split * s.batch * s.kv_heads + bh) * rows + row;
-        if (half == 0) a.part_l[pat] = some ? lse : (exists && l != l ? l : -INFINITY);
+        if (half == 0) a.part_l[pat] = lse == INFINITY ? -INFINITY : lse;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnFwd<T> a) {
             if (e < left) v[e] = fmaf(w, p[e], v[e]);
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (a.lse && c == 0) a.lse[at] = sum > 0.f ? use + log2f(sum) : INFINITY;
+    if (a.lse && c == 0) a.lse[at] = sum == 0.f ? INFINITY : use + log2f(sum);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= inv;
     const int i0 = row_point(s, row);

@@ -62,3 +62,29 @@ def test_sizes_beyond_32_bits_are_refused():
     row = torch.empty(1, 2 ** 32 + 8, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(RuntimeError, match="range"):
         torch.ops.equigspr.residual_norm(row, row, None, None, None, None, None, None, False, 1e-5, 1.0, 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("nq,nk,causal", [(40, 150, False), (3, 5000, False), (130, 130, True)])
+def test_attention_nan_in_a_seen_key_reaches_every_gradient(dtype, nq, nk, causal):
+    """NaN in one key of one key head that every point sees (a row's sum is then NaN): its query heads' outputs and all gradients of that
+    head are NaN, those of the other head and of keys behind the length are untouched.  The key axis whole and split."""
+    g = torch.Generator().manual_seed(44)
+    q, k, v, go = (normal(g, 2, n, h, 16, dtype=dtype) for n, h in ((nq, 4), (nk, 2), (nk, 2), (nq, 4)))
+    kl = torch.tensor([nk, nk - 1], dtype=torch.int32)
+
+    def run(poison):
+        t = [q.clone(), k.clone(), v.clone()]
+        if poison:
+            t[1][1, 0, 1, 3] = float("nan")                                # sample 1, first key (seen by all, causal too), head 1
+        a = [x.cuda().requires_grad_(True) for x in t]
+        out = pkg().cloud_attention(*a, kv_lens=None if causal else kl.cuda(), causal=causal)
+        return [out.detach()] + list(torch.autograd.grad(out, a, go.cuda()))
+    clean, dirty = run(False), run(True)
+    last = nk if causal else nk - 1
+    for i, (c, d) in enumerate(zip(clean, dirty)):
+        heads = slice(2, 4) if i in (0, 1) else slice(1, 2)
+        rest = slice(0, 2) if i in (0, 1) else slice(0, 1)
+        n = c.shape[1] if i in (0, 1) else last
+        assert d[1, :n, heads].isnan().all(), i
+        assert torch.equal(c[0], d[0]) and torch.equal(c[1, :, rest], d[1, :, rest]) and torch.equal(c[1, n:], d[1, n:]), i
