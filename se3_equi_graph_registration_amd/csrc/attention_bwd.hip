@@ -35,7 +35,7 @@ struct AttnBwd {
 // rows of a staged tile: 64, or 32 where three planes or a wide head would take the registers of a second wave per SIMD
 template <int T, int W> constexpr int attn_bwd_tile() { return W == 128 || (T == kF32 && W == 64) ? 32 : 64; }
 
-// fp16: largest |dO| over the existing rows and |V| over the visible keys, one pair per workgroup
+// fp16: largest |dO| over the rows with a visible key and |V| over the visible keys, one pair per workgroup
 template <int T>
 __global__ __launch_bounds__(256) void attn_amax_kernel(AttnBwd<T> a) {
     const AttnShape& s = a.s;
@@ -53,7 +53,9 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(AttnBwd<T> a) {
     for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < ng * per_g; id += kAmaxBlocks * 256) {
         const int64_t pt = id / per_g;
         const int hc = (int)(id - pt * per_g), h = hc / chunks, b = (int)(pt / s.nq), i = (int)(pt - (int64_t)b * s.nq);
-        if (i < attn_len(s.q_lens, b, s.nq)) most(mg, a.g.p + b * a.g.sb + i * a.g.sn + h * a.g.sh, hc - h * chunks);
+        const int hk = h / s.group;
+        const bool some = i < attn_len(s.q_lens, b, s.nq) && a.lse[((int64_t)b * s.kv_heads + hk) * s.nq * s.group + i * s.group + h - hk * s.group] != INFINITY;
+        if (some) most(mg, a.g.p + b * a.g.sb + i * a.g.sn + h * a.g.sh, hc - h * chunks);
     }
     for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < nv * per_v; id += kAmaxBlocks * 256) {
         const int64_t pt = id / per_v;
@@ -112,6 +114,9 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_ker
     const uint8_t* mask = s.key_mask ? s.key_mask + b * s.mask_stride : nullptr;
     const int64_t at = (int64_t)bh * rows + row;
 
+    // A row without a visible key takes no gradient, whatever it and its output gradient hold: both become zeros (after their loads, which
+    // need not wait for the log-sum).
+    const float lse = ok_row ? a.lse[at] : INFINITY;
     Op8<T> q[KS], g[KS];
     float delta = 0.f;
     {
@@ -121,8 +126,10 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_ker
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int c = ks * 16 + half * 8;
-            q[ks] = planes_of<T>(ok_row ? load8<T>(pq, c, s.dim) : raw_zero<T>());
-            const Raw8<T> rg = ok_row ? load8<T>(pg, c, s.dim) : raw_zero<T>(), ro = ok_row ? load8<T>(po, c, s.dim) : raw_zero<T>();
+            Raw8<T> rq = ok_row ? load8<T>(pq, c, s.dim) : raw_zero<T>(), rg = ok_row ? load8<T>(pg, c, s.dim) : raw_zero<T>();
+            const Raw8<T> ro = ok_row ? load8<T>(po, c, s.dim) : raw_zero<T>();
+            if (lse == INFINITY) rq = rg = raw_zero<T>();
+            q[ks] = planes_of<T>(rq);
 #pragma unroll
             for (int i = 0; i < 8; ++i) delta = fmaf(raw_float<T>(rg, i), raw_float<T>(ro, i), delta);
             if (T != kF32 && a.o_low && ok_row) {
@@ -136,7 +143,6 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_ker
     delta += __shfl_xor(delta, 32);
     if (row < rows && half == 0 && split == 0) a.delta[at] = delta;
     if (!a.gq) return;
-    const float lse = ok_row ? a.lse[at] : INFINITY;
     const float factor = attn_grad_scale<T>(a);
     pf32x16 acc[DB];
 #pragma unroll
@@ -286,6 +292,12 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dkv_ke
         } else {
             sq.load([&](int r) { return r0 + r < r_end ? packed_row(a.q, s, b, hk, r0 + r) : nullptr; }, s.dim);
             sg.load([&](int r) { return r0 + r < r_end ? packed_row(a.g, s, b, hk, r0 + r) : nullptr; }, s.dim);
+        }
+        // Rows without a visible key among the rows of this tile's keys (there are none unless a mask hides what causal leaves).
+        if (s.key_mask && s.causal) {
+            auto gone = [&](int r) { return r0 + r < r_end && a.lse[(int64_t)bh * rows + r0 + r] == INFINITY; };
+            sq.drop(gone);
+            sg.drop(gone);
         }
         if (threadIdx.x < RT) {
             const int r = r0 + threadIdx.x;

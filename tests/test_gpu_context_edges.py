@@ -88,3 +88,34 @@ def test_attention_nan_in_a_seen_key_reaches_every_gradient(dtype, nq, nk, causa
         n = c.shape[1] if i in (0, 1) else last
         assert d[1, :n, heads].isnan().all(), i
         assert torch.equal(c[0], d[0]) and torch.equal(c[1, :, rest], d[1, :, rest]) and torch.equal(c[1, n:], d[1, n:]), i
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("nq,nk,causal,hidden,heads", [(70, 90, False, 90, (4, 2)), (100, 100, True, 30, (4, 2)), (600, 600, True, 130, (3, 1)), (90, 40, True, 0, (2, 2))])
+def test_attention_points_without_a_key_take_no_gradient(dtype, nq, nk, causal, hidden, heads):
+    """NaN and infinities in the points that see no key, and in their output gradients: the results of finite ones, zeros for those points.
+    Nothing visible at all; a mask over the first keys under causal; more points than keys under causal."""
+    g = torch.Generator().manual_seed(45)
+    h, hk = heads
+    q, k, v, go = (normal(g, 2, n, e, 24, dtype=dtype) for n, e in ((nq, h), (nk, hk), (nk, hk), (nq, h)))
+    mask = None
+    if hidden:
+        mask = torch.ones(2, nk, dtype=torch.bool)
+        mask[1, :hidden] = False
+    dead = ~orc.visible(2, nq, nk, None, None, mask, causal).any(-1)
+    assert dead.any()
+
+    def run(poison):
+        t = [x.clone() for x in (q, k, v, go)]
+        if poison:
+            bad = torch.tensor([float("nan"), float("inf"), float("-inf")], dtype=dtype)
+            for x in (t[0], t[3]):
+                x[dead] = bad[torch.arange(int(dead.sum())) % 3][:, None, None]
+        a = [x.cuda().requires_grad_(True) for x in t[:3]]
+        out = pkg().cloud_attention(*a, key_mask=None if mask is None else mask.cuda(), causal=causal)
+        return [out.detach()] + list(torch.autograd.grad(out, a, t[3].cuda()))
+    clean, dirty = run(False), run(True)
+    for i, (c, d) in enumerate(zip(clean, dirty)):
+        assert torch.equal(c, d), i
+    for i in (0, 1):
+        assert float(dirty[i][dead.cuda()].abs().max()) == 0.0
