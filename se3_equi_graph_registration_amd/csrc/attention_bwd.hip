@@ -10,12 +10,11 @@
 // Bound: as the forward, and the registers -- the accumulators of wide heads leave two waves per SIMD.  Measured, bf16: 8 x 2048^2 x 8 heads
 // of 64 340 us (505 TFLOP/s of the five products that the mathematics needs), 8192^2 x 16 / 4 heads of 128 2.0 ms (680), causal 1.14 ms.
 // fp16: dS is about 1/keys of the output gradient and would sink below fp16's range, so it is held as 2^E dS, with E from the largest
-// |dO| and |V| such that the bound |dS| <= 2 dim max|dO| max|V| stays in range; undone in fp32 at the end.
+// |dO| and |V| of the sample and key head such that the bound |dS| <= 2 dim max|dO| max|V| stays in range; undone in fp32 at the end.
+// (One E for a whole batch would let one sample's or head's large gradients push the others' into fp16's smallest steps.)
 #include "attention_device.h"
 
 namespace eq {
-
-constexpr int kAmaxBlocks = 1024;
 
 template <int T>
 struct AttnBwd {
@@ -24,7 +23,8 @@ struct AttnBwd {
     const typename Num<T>::type* o_low;       // 16-bit types: what the output's rounding dropped, or null
     const float* lse;
     float* delta;                             // [batch, kv_heads, nq * group]
-    float* amax;                              // fp16: [2 * kAmaxBlocks]
+    float* amax;                              // fp16: [batch * kv_heads][amax_parts][2], largest |dO| and |V|
+    int amax_parts;                           // <= 64
     typename Num<T>::type *gq, *gk, *gv;      // contiguous, each may be null
     int row_tiles, key_tiles;
     int key_splits, split_keys;               // attn_dq_kernel: parts of the key axis
@@ -35,32 +35,26 @@ struct AttnBwd {
 // rows of a staged tile: 64, or 32 where three planes or a wide head would take the registers of a second wave per SIMD
 template <int T, int W> constexpr int attn_bwd_tile() { return W == 128 || (T == kF32 && W == 64) ? 32 : 64; }
 
-// fp16: largest |dO| over the rows with a visible key and |V| over the visible keys, one pair per workgroup
+// fp16: largest |dO| over the rows with a visible key and |V| over the visible keys of a sample and key head, one pair per workgroup
 template <int T>
 __global__ __launch_bounds__(256) void attn_amax_kernel(AttnBwd<T> a) {
     const AttnShape& s = a.s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int bh = blockIdx.x / a.amax_parts, at = blockIdx.x - bh * a.amax_parts, b = bh / s.kv_heads, hk = bh - b * s.kv_heads;
     float mg = 0.f, mv = 0.f;
-    const int chunks = (s.dim + 7) / 8;
-    auto most = [&](float& m, const typename Num<T>::type* row, int c) {
+    // a thread per chunk of eight values: as many whole rows at a time as fit the workgroup
+    const int chunks = (s.dim + 7) / 8, per = 256 / chunks, r0 = threadIdx.x / chunks, c = threadIdx.x - r0 * chunks;
+    auto most = [&](float& m, const typename Num<T>::type* row) {
         const Raw8<T> r = load8<T>(row, 8 * c, s.dim);
 #pragma unroll
         for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(raw_float<T>(r, i)));
     };
-    // a thread per chunk of eight values
-    const int64_t ng = (int64_t)s.batch * s.nq, nv = (int64_t)s.batch * s.nk;
-    const int per_g = s.heads * chunks, per_v = s.kv_heads * chunks;
-    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < ng * per_g; id += kAmaxBlocks * 256) {
-        const int64_t pt = id / per_g;
-        const int hc = (int)(id - pt * per_g), h = hc / chunks, b = (int)(pt / s.nq), i = (int)(pt - (int64_t)b * s.nq);
-        const int hk = h / s.group;
-        const bool some = i < attn_len(s.q_lens, b, s.nq) && a.lse[((int64_t)b * s.kv_heads + hk) * s.nq * s.group + i * s.group + h - hk * s.group] != INFINITY;
-        if (some) most(mg, a.g.p + b * a.g.sb + i * a.g.sn + h * a.g.sh, hc - h * chunks);
-    }
-    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < nv * per_v; id += kAmaxBlocks * 256) {
-        const int64_t pt = id / per_v;
-        const int hc = (int)(id - pt * per_v), h = hc / chunks, b = (int)(pt / s.nk), j = (int)(pt - (int64_t)b * s.nk);
-        if (j < attn_len(s.kv_lens, b, s.nk) && (!s.key_mask || s.key_mask[b * s.mask_stride + j])) most(mv, key_row(a.v, b, h, j), hc - h * chunks);
+    const int rows = attn_len(s.q_lens, b, s.nq) * s.group, keys = attn_len(s.kv_lens, b, s.nk);
+    if (r0 < per) {
+        for (int r = at * per + r0; r < rows; r += a.amax_parts * per)
+            if (a.lse[(int64_t)bh * s.nq * s.group + r] != INFINITY) most(mg, packed_row(a.g, s, b, hk, r));
+        for (int j = at * per + r0; j < keys; j += a.amax_parts * per)
+            if (!s.key_mask || s.key_mask[b * s.mask_stride + j]) most(mv, key_row(a.v, b, hk, j));
     }
     __shared__ float part[2][4];
     for (int o = 32; o; o >>= 1) { mg = fmaxf(mg, __shfl_xor(mg, o)); mv = fmaxf(mv, __shfl_xor(mv, o)); }
@@ -69,17 +63,19 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(AttnBwd<T> a) {
     if (threadIdx.x < 2)
         a.amax[2 * blockIdx.x + threadIdx.x] = fmaxf(fmaxf(part[threadIdx.x][0], part[threadIdx.x][1]), fmaxf(part[threadIdx.x][2], part[threadIdx.x][3]));
 }
+// enough workgroups for the card when there are few heads; a wave joins a head's parts with one load
+static int attn_amax_parts(int64_t heads) { return heads >= 1024 ? 1 : heads <= 16 ? 64 : (int)(1024 / heads); }
 
 // the power of two dS is held with: 1 except in fp16
 template <int T>
-__device__ __forceinline__ float attn_grad_scale(const AttnBwd<T>& a) {
+__device__ __forceinline__ float attn_grad_scale(const AttnBwd<T>& a, int bh) {
     if constexpr (T != kF16) return 1.f;
     const int lane = threadIdx.x & 63;
     float mg = 0.f, mv = 0.f;
-#pragma unroll
-    for (int i = 0; i < kAmaxBlocks / 64; ++i) {
-        mg = fmaxf(mg, a.amax[2 * (lane + 64 * i)]);
-        mv = fmaxf(mv, a.amax[2 * (lane + 64 * i) + 1]);
+    if (lane < a.amax_parts) {
+        const float* p = a.amax + 2 * ((int64_t)bh * a.amax_parts + lane);
+        mg = p[0];
+        mv = p[1];
     }
     for (int o = 32; o; o >>= 1) { mg = fmaxf(mg, __shfl_xor(mg, o)); mv = fmaxf(mv, __shfl_xor(mv, o)); }
     const float bound = 2.f * a.s.dim * mg * mv;
@@ -143,7 +139,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dq_ker
     delta += __shfl_xor(delta, 32);
     if (row < rows && half == 0 && split == 0) a.delta[at] = delta;
     if (!a.gq) return;
-    const float factor = attn_grad_scale<T>(a);
+    const float factor = attn_grad_scale<T>(a, bh);
     pf32x16 acc[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -272,7 +268,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, T == kF32 ? 1 : 2) void attn_dkv_ke
             else *reinterpret_cast<s16x8*>(own_v + Tile<W>::at(wave * 32 + (lane & 31), 2 * ks + half)) = o.p[0];
         }
     }
-    const float factor = attn_grad_scale<T>(a), fs = factor * exp2_fast(-kShift);
+    const float factor = attn_grad_scale<T>(a, bh), fs = factor * exp2_fast(-kShift);
     pf32x16 acc_k[DB], acc_v[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -419,7 +415,7 @@ static int attn_bwd_splits(int64_t tiles, int64_t length, int64_t want) {
     return (int)(s < most ? (s > 1 ? s : 1) : (most > 1 ? most : 1));
 }
 
-struct AttnBwdPlan { int row_tiles, key_tiles, key_splits, split_keys, row_splits; int64_t delta, parts_q, parts_k; };
+struct AttnBwdPlan { int row_tiles, key_tiles, key_splits, split_keys, row_splits; int amax_parts; int64_t amax, delta, parts_q, parts_k; };
 static AttnBwdPlan attn_bwd_plan(const AttnShape& s) {
     constexpr int kOwned = kBwdWaves * 32;
     AttnBwdPlan p;
@@ -430,6 +426,8 @@ static AttnBwdPlan attn_bwd_plan(const AttnShape& s) {
     p.split_keys = ceil_div(ceil_div(s.nk, p.key_splits), 64) * 64;
     p.key_splits = s.nk ? ceil_div(s.nk, p.split_keys) : 1;
     p.row_splits = attn_bwd_splits(p.key_tiles * heads, rows, s.causal ? 1024 : 512);
+    p.amax_parts = attn_amax_parts(heads);
+    p.amax = (2 * heads * p.amax_parts + 3) / 4 * 4;
     p.delta = (heads * rows + 3) / 4 * 4;
     p.parts_q = p.key_splits > 1 ? p.key_splits * heads * rows * s.dim : 0;
     p.parts_k = p.row_splits > 1 ? p.row_splits * heads * s.nk * s.dim : 0;
@@ -443,7 +441,7 @@ static int attn_bwd_launch(const AttnBwd<T>& a, hipStream_t st) {
     const int64_t bq = (int64_t)a.row_tiles * a.key_splits * heads, bk = (int64_t)a.key_tiles * a.row_splits * heads;
     EQ_CHECK_ARG(bq < (1 << 24) && bk < (1 << 24), EQUIGSPR_ENOTSUP, "attention_backward: more workgroups than one launch takes");
     if (T == kF16) {
-        attn_amax_kernel<T><<<kAmaxBlocks, 256, 0, st>>>(a);
+        attn_amax_kernel<T><<<(unsigned)(heads * a.amax_parts), 256, 0, st>>>(a);
         EQ_CHECK_LAUNCH("attention_backward (range)");
     }
     if (bq) {
@@ -483,7 +481,8 @@ static int attn_bwd(const equigspr_attention* d, const AttnShape& s, const void*
     a.lse = lse;
     a.amax = work;
     const AttnBwdPlan p = attn_bwd_plan(s);
-    a.delta = work + 2 * kAmaxBlocks;
+    a.amax_parts = p.amax_parts;
+    a.delta = work + p.amax;
     a.part_q = a.part_k = a.delta + p.delta;  // the rows' parts are summed before the keys' parts are written
     a.part_v = a.part_k + p.parts_k;
     a.row_tiles = p.row_tiles; a.key_tiles = p.key_tiles; a.key_splits = p.key_splits; a.split_keys = p.split_keys; a.row_splits = p.row_splits;
@@ -497,7 +496,7 @@ extern "C" int64_t equigspr_attention_backward_work_size(const equigspr_attentio
     eq::AttnShape s;
     if (eq::attn_shape(d, &s) != 0) return -1;
     const eq::AttnBwdPlan p = eq::attn_bwd_plan(s);
-    return 2 * eq::kAmaxBlocks + p.delta + (p.parts_q > 2 * p.parts_k ? p.parts_q : 2 * p.parts_k);
+    return p.amax + p.delta + (p.parts_q > 2 * p.parts_k ? p.parts_q : 2 * p.parts_k);
 }
 
 extern "C" int equigspr_attention_backward(const equigspr_attention* d, const void* out, const void* out_low, const float* lse,

@@ -119,3 +119,22 @@ def test_attention_points_without_a_key_take_no_gradient(dtype, nq, nk, causal, 
         assert torch.equal(c, d), i
     for i in (0, 1):
         assert float(dirty[i][dead.cuda()].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_fp16_gradients_do_not_depend_on_their_neighbours(causal):
+    """Samples and heads whose output gradients and values are of very different sizes: each keeps the accuracy it has alone (its bound is
+    the oracle's for that sample and key head by itself)."""
+    g = torch.Generator().manual_seed(46)
+    dt, n, d = torch.float16, 1500, 32
+    q, k, v, go = (normal(g, 2, n, h, d, dtype=dt) for h in (4, 2, 2, 4))
+    go = (go.float() * torch.tensor([[1e4, 1e-3], [1.0, 1e-2]]).repeat_interleave(2, 1)[:, None, :, None]).to(dt)
+    v = (v.float() * torch.tensor([1.0, 0.25])[None, None, :, None]).to(dt)
+    a = [x.cuda().requires_grad_(True) for x in (q, k, v)]
+    out = pkg().cloud_attention(*a, causal=causal)
+    got = dict(zip(("grad_q", "grad_k", "grad_v"), torch.autograd.grad(out, a, go.cuda())), out=out)
+    for b in range(2):
+        for e in range(2):
+            rows, keys = (slice(b, b + 1), slice(None), slice(2 * e, 2 * e + 2)), (slice(b, b + 1), slice(None), slice(e, e + 1))
+            val, err = orc.attention(q[rows], k[keys], v[keys], go[rows], causal=causal)
+            within({m: t[rows if m in ("out", "grad_q") else keys] for m, t in got.items()}, val, err, f"attention fp16, sample {b}, key head {e}")
