@@ -9,6 +9,7 @@
 // is ever transposed in memory.  Products accumulate in fp32.  h, dz and du are operands of further products and are stored in the
 // inputs' type (one rounding each); z | u, which only the epilogue of the backward reads, stays fp32 -- in 16 bits its rounding would come
 // on top of dz's and du's in every gradient (bf16: 1.8 instead of 1.4 times the outputs' own rounding).
+// fp16: dz and du are held as 2^E dz and 2^E du, with E from the largest |dy| (ff_held), undone in fp32 where their products leave.
 // Bound: the matrix pipe for many rows, the weights' bytes for few.  Measured, bf16, 16384 x 1024 x 4096: projections 402 us (685 TFLOP/s,
 // with 0.7 GB of results), output 147 (935), hidden gradients 330 (415, with 0.8 GB through its epilogue), input 276 (995), weights 300 + 161 (915, 855).
 #include "planes.h"
@@ -40,12 +41,45 @@ struct FfArgs {
     float* part;                              // [cuts][m][n]
     float* zu;                                // kGate: written if not null; kGrad: read.  [m, 2 n]
     E* dzu;                                   // kGrad: [m, 2 n]
+    const float* range;                       // fp16 backward: [kFfRange], largest |dy|; kGrad scales dz | du by ff_held, kPlain divides by it.  Null: 1
     int act;
 };
 
 __device__ __forceinline__ void floats_of(const Raw8<kF32>& r, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = raw_float<kF32>(r, i);
+}
+
+// fp16: the power of two that dz and du are held with, so that output gradients far below 1 do not sink into fp16's smallest steps and
+// far larger ones do not leave its range.  1 while the largest |dy| lies in [2^-4, 2^4); otherwise it brings that to [2^-4, 2^-3) or [2^3, 2^4):
+// dz and du may then be 2^12 times it, and keep all their bits down to 2^-10 of it.
+constexpr int kFfRange = 256;                 // workgroups that look for the largest |dy|
+template <int T>
+__device__ __forceinline__ float ff_held(const float* range) {
+    if constexpr (T != kF16) return 1.f;
+    if (!range) return 1.f;
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < kFfRange / 64; ++i) m = fmaxf(m, range[(threadIdx.x & 63) + 64 * i]);
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if (!(m > 0.f) || m == INFINITY) return 1.f;
+    const int e = ilogbf(m);
+    return ldexpf(1.f, e < -4 ? -4 - e : e >= 4 ? 3 - e : 0);
+}
+template <int T>
+__global__ __launch_bounds__(256) void ff_range_kernel(const typename Num<T>::type* x, int64_t n, float* range) {
+    float m = 0.f;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)kFfRange * 256 * 8) {
+        float v[8];
+        load8f<T>(x + i, n - i < 8 ? (int)(n - i) : 8, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]));
+    }
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    __shared__ float part[4];
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) range[blockIdx.x] = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
 }
 
 // act(z) and its derivative
@@ -271,6 +305,7 @@ __global__ __launch_bounds__((FfShapeOf<T, kLarge>::kThreads), 2) void ff_produc
         }
     }
     __syncthreads();                              // the last tiles have been read
+    const float held = kEpi == kGate ? 1.f : ff_held<T>(g.range), back = 1.f / held;
     float* const out = reinterpret_cast<float*>(lds) + wave * kOutFloats;
     constexpr int kCols = kEpi == kGate ? 32 : 64, kLanes = kCols / 8, kRows = 64 / kLanes;      // columns, lanes per row, rows of a step
     const int col = n0 + (kEpi == kGate ? wn * 32 : wn * 64) + lane % kLanes * 8, left = g.n - col;
@@ -335,6 +370,7 @@ __global__ __launch_bounds__((FfShapeOf<T, kLarge>::kThreads), 2) void ff_produc
                 for (int e = 0; e < 8; ++e) {
                     float a, d;
                     activate(g.act, z[e], a, d);
+                    if constexpr (T == kF16) v[e] *= held;
                     z[e] = v[e] * u[e] * d;
                     u[e] = v[e] * a;
                 }
@@ -343,6 +379,10 @@ __global__ __launch_bounds__((FfShapeOf<T, kLarge>::kThreads), 2) void ff_produc
             } else if (g.cuts > 1) {
                 store8<kF32>(g.part + ((int64_t)cut * g.m + row) * g.n + col, v, left);
             } else {
+                if constexpr (T == kF16) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] *= back;
+                }
                 if (g.bias) {
                     load8f<T>(g.bias + col, left, z);
 #pragma unroll
@@ -462,10 +502,12 @@ __global__ __launch_bounds__(kFewWaves * 64) void ff_few_kernel(FfArgs<T> g) {
 template <int T>
 __global__ __launch_bounds__(256) void ff_sum_kernel(FfArgs<T> g) {
     const int64_t n = (int64_t)g.m * g.n;
+    const float back = 1.f / ff_held<T>(g.range);      // 1 wherever there is a bias
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         float v = g.bias ? (float)g.bias[i % g.n] : 0.f;
 #pragma unroll 8
         for (int c = 0; c < g.cuts; ++c) v += g.part[c * n + i];
+        if constexpr (T == kF16) v *= back;
         store_value<T>(g.c + i, v);
     }
 }
@@ -478,6 +520,7 @@ struct FfColumns {
     typename Num<T>::type* out[2];
     int width[2];                             // 0: not wanted
     int rows, runs;
+    const float* range;                       // fp16: as FfArgs::range, for x[0]
 };
 constexpr int kFfRun = 128;                   // rows of a run
 template <int T>
@@ -502,6 +545,7 @@ template <int T>
 __global__ __launch_bounds__(256) void ff_columns_sum_kernel(FfColumns<T> a, const float* part) {
     const int all = a.width[0] + a.width[1], c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
     __shared__ float lds[4][64];
+    const float back = 1.f / ff_held<T>(a.range);
     float v = 0.f;
     if (c < all)
 #pragma unroll 8
@@ -510,7 +554,7 @@ __global__ __launch_bounds__(256) void ff_columns_sum_kernel(FfColumns<T> a, con
     __syncthreads();
     if (q || c >= all) return;
     v = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
-    if (c < a.width[0]) store_value<T>(a.out[0] + c, v);
+    if (c < a.width[0]) store_value<T>(a.out[0] + c, T == kF16 ? v * back : v);
     else store_value<T>(a.out[1] + c - a.width[0], v);
 }
 
@@ -616,6 +660,14 @@ static int ff_backward(const equigspr_gated_feed_forward* d, const void* gy, con
     const int r = d->rows, w = d->width, hd = d->hidden, out = d->out;
     FfArgs<T> g = {};
     g.act = d->activation;
+    const float* range = nullptr;
+    if constexpr (T == kF16) {                // the first floats of the workspace
+        ff_range_kernel<T><<<kFfRange, 256, 0, st>>>((const E*)gy, (int64_t)r * out, work);
+        EQ_CHECK_LAUNCH("gated_feed_forward_backward (range)");
+        range = work;
+        work += kFfRange;
+    }
+    g.range = range;
     // dh = dy Wd: rows of dy along the contraction (out), Wd [out, hidden] across it
     g.a = ff_operand<T>(gy, r, out);
     g.b = ff_operand<T>(d->w_down, out, hd);
@@ -645,12 +697,13 @@ static int ff_backward(const equigspr_gated_feed_forward* d, const void* gy, con
         g.a = ff_operand<T>(gy, r, out);
         g.b = ff_operand<T>(h, r, hd);
         g.m = out; g.n = hd; g.k = r;
+        g.range = nullptr;
         g.c = (E*)o->grad_w_down;
         if (const int rc = ff_product<T, true, true, kPlain>(g, st, "gated_feed_forward_backward (output)")) return rc;
     }
     if (o->grad_b_gate_up || o->grad_b_down) {
         FfColumns<T> c = {{(const E*)dzu, (const E*)gy}, {(E*)o->grad_b_gate_up, (E*)o->grad_b_down}, {o->grad_b_gate_up ? 2 * hd : 0, o->grad_b_down ? out : 0},
-                          r, ceil_div(r, kFfRun)};
+                          r, ceil_div(r, kFfRun), range};
         ff_columns_kernel<T><<<dim3(ceil_div(c.width[0], 64) + ceil_div(c.width[1], 64), c.runs), 256, 0, st>>>(c, work);
         EQ_CHECK_LAUNCH("gated_feed_forward_backward (biases)");
         ff_columns_sum_kernel<T><<<ceil_div(c.width[0] + c.width[1], 64), 256, 0, st>>>(c, work);
@@ -695,7 +748,7 @@ extern "C" int64_t equigspr_gated_feed_forward_backward_work_size(const equigspr
     const int64_t sums = (int64_t)eq::ceil_div(d->rows, eq::kFfRun) * (2 * d->hidden + d->out);
     n = up > n ? up : n;
     n = down > n ? down : n;
-    return sums > n ? sums : n;
+    return (sums > n ? sums : n) + (d->dtype == EQUIGSPR_F16 ? eq::kFfRange : 0);
 }
 
 extern "C" int equigspr_gated_feed_forward_backward(const equigspr_gated_feed_forward* d, const void* grad_y, const float* zu, const void* h, void* dzu, float* work,

@@ -16,8 +16,9 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
     ``x [..., width]``, ``w_gate`` and ``w_up [hidden, width]``, ``w_down [out, hidden]`` (the layout of ``nn.Linear``), biases optional:
     float32, bfloat16 or float16, all alike, on one device (tensors that are not contiguous are copied).  ``activation``: "silu", "gelu"
     (exact) or "relu".  Products accumulate in fp32; the hidden layer is held in the inputs' dtype between the two products, as are the
-    projections' gradients in the backward: in float16 they must stay within that type's range.  The backward keeps both projections in
-    float32.  Up to 8 388 480 rows a call.  Differentiable once in every
+    projections' gradients in the backward.  In float16 the hidden layer must stay within that type's range; the projections' gradients are
+    held relative to the largest output gradient, must stay within 2^12 times it and lose bits below 2^-10 of it.  The backward keeps both
+    projections in float32.  Up to 8 388 480 rows a call.  Differentiable once in every
     tensor (reverse mode; tangents are refused); bitwise reproducible (no atomics)."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"gated_feed_forward: activation {activation!r}, expected one of {sorted(ACTIVATIONS)}")

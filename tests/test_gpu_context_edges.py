@@ -138,3 +138,42 @@ def test_attention_fp16_gradients_do_not_depend_on_their_neighbours(causal):
             rows, keys = (slice(b, b + 1), slice(None), slice(2 * e, 2 * e + 2)), (slice(b, b + 1), slice(None), slice(e, e + 1))
             val, err = orc.attention(q[rows], k[keys], v[keys], go[rows], causal=causal)
             within({m: t[rows if m in ("out", "grad_q") else keys] for m, t in got.items()}, val, err, f"attention fp16, sample {b}, key head {e}")
+
+
+@pytest.mark.parametrize("rows", [20, 64])
+def test_feed_forward_fp16_gradients_of_any_size(rows):
+    """fp16 output gradients far below 1 (products of the hidden layer's gradients would sink into the type's smallest steps) and far above
+    (they would leave its range)."""
+    g = torch.Generator().manual_seed(47)
+    dt, width, hidden = torch.float16, 32, 48
+    x = normal(g, rows, width, dtype=dt, scale=64.0)
+    t = {"x": x, "w_gate": normal(g, hidden, width, dtype=dt, scale=width ** -0.5 / 64), "w_up": normal(g, hidden, width, dtype=dt, scale=width ** -0.5 / 64),
+         "w_down": normal(g, width, hidden, dtype=dt, scale=2.0 ** -5), "b_gate": normal(g, hidden, dtype=dt), "b_up": normal(g, hidden, dtype=dt)}
+    k = torch.randint(-512, 513, (rows, width), generator=g)
+    k[0, 0] = 512
+    small = (k * 2.0 ** -24).to(dt)                                        # exact: whole steps of fp16, up to 2^-15
+    dev = {n: v.cuda().requires_grad_(True) for n, v in t.items()}
+    y = pkg().gated_feed_forward(**dev)
+    got = {"grad_" + n: v.double().cpu() * 2.0 ** 11 for n, v in zip(dev, torch.autograd.grad(y, list(dev.values()), small.cuda(), retain_graph=True))}
+    # the same gradients times 2^11 (largest 2^-4): dz and du are held as if the call had been given these; the results' own smallest step
+    # is 2^11 times as large in these units
+    val, err = orc.feed_forward(**t, grad=(k * 2.0 ** -13).to(dt))
+    within(got, val, {n: e + 2.0 ** -14 for n, e in err.items()}, "feed_forward fp16, small gradients")
+    # large: |grad| up to 2^15, dz and du up to 2^15 * 2^4 if they were held as they are.  What x and the weights bring down stays in range.
+    t.update(x=normal(g, rows, width, dtype=dt, scale=2.0 ** -7), w_down=normal(g, width, hidden, dtype=dt, scale=1.0),
+             b_up=normal(g, hidden, dtype=dt, scale=4.0))
+    large = (k * 2.0 ** 6).to(dt)
+    dev = {n: v.cuda().requires_grad_(True) for n, v in t.items()}
+    names = ["x", "w_gate", "w_up"]
+    got = dict(zip(["grad_" + n for n in names], torch.autograd.grad(pkg().gated_feed_forward(**dev), [dev[n] for n in names], large.cuda())))
+    val, err = orc.feed_forward(**t, grad=large)
+    # held as 2^E dz, 2^E = 2^-12 for a largest |grad| of 2^15: the steps below fp16's normal range are 2^12 times the oracle's 2^-25, and
+    # enter the results through the absolute sums of the other operand
+    step = 2.0 ** (12 - 25)
+    floor = {"grad_x": step * (t["w_gate"].double().abs().sum(0) + t["w_up"].double().abs().sum(0)).expand(rows, -1),
+             "grad_w_gate": step * t["x"].double().abs().sum(0).expand(hidden, -1), "grad_w_up": step * t["x"].double().abs().sum(0).expand(hidden, -1)}
+    for n in got:                                                          # a result beyond fp16's range is infinite, not compared
+        bound = err[n] + floor[n]
+        g16, beyond, inside = got[n].cpu().double(), val[n].abs() - bound > 65520, val[n].abs() + bound < 65504
+        assert (g16[beyond] == val[n].sign()[beyond] * float("inf")).all() and inside.sum() > 0.9 * inside.numel(), n
+        within({n: torch.where(inside, g16, 0.0)}, {n: torch.where(inside, val[n], 0.0)}, {n: bound}, "feed_forward fp16, large gradients")
