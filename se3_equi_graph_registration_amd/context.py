@@ -17,7 +17,8 @@ from .norms import ResidualNorm
 class CloudContext(nn.Module):
     """``forward(h [2, B, N, width], valid=None) -> [2, B, N, width]``: ``h[0]`` / ``h[1]`` the point features of the source / target clouds.
     ``valid`` (bool ``[2, B, N]``): points that exist; the others are not looked at.  ``residual_scale`` starts the blocks near the
-    identity."""
+    identity.  The blocks run in the type of their parameters (``CloudContext(...).bfloat16()`` behind an fp32 EGNN), or, their products, in
+    that of ``torch.autocast``; the result has the type of ``h``."""
 
     def __init__(self, width, n_layers=1, num_heads=4, hidden=None, kind="layer", activation="silu", residual_scale=0.1, device="cuda:0"):
         super().__init__()
@@ -41,11 +42,11 @@ class CloudContext(nn.Module):
             raise RuntimeError(f"valid: expected bool [2, {b}, {n}], got {valid.dtype} {tuple(valid.shape)}")
         mask = None if valid is None else valid.reshape(2 * b, n)
         other_mask = None if valid is None else valid.flip(0).reshape(2 * b, n)
-        x = h.reshape(2 * b, n, c)
+        x = h.reshape(2 * b, n, c).to(self.first.pre_weight.dtype)
         _, u = self.first(x)
         step = iter(self.steps)
         for i in range(self.n_layers):
             x, u = next(step)(x, self.self_attention[i](u, key_mask=mask))
             x, u = next(step)(x, self.cross_attention[i](u, torch.cat([u[b:], u[:b]]), key_mask=other_mask))
             x, u = next(step)(x, self.feed_forward[i](u))
-        return x.view(2, b, n, c)
+        return x.view(2, b, n, c).to(h.dtype)

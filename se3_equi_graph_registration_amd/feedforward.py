@@ -5,7 +5,7 @@ from __future__ import annotations
 
 from torch import nn
 
-from .ops import context_ops, need_float
+from .ops import autocast_type, context_ops, need_float
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}      # EQUIGSPR_ACT_*
 
@@ -41,7 +41,8 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
 
 
 class GatedFeedForward(nn.Module):
-    """``gated_feed_forward`` with its parameters: ``gate`` and ``up`` (width -> hidden), ``down`` (hidden -> width)."""
+    """``gated_feed_forward`` with its parameters: ``gate`` and ``up`` (width -> hidden), ``down`` (hidden -> width).  Under ``torch.autocast``
+    the block runs in its type, as ``nn.Linear`` does."""
 
     def __init__(self, width, hidden, activation="silu", bias=True):
         super().__init__()
@@ -52,5 +53,8 @@ class GatedFeedForward(nn.Module):
         self.down = nn.Linear(hidden, width, bias=bias)
 
     def forward(self, x):
-        return gated_feed_forward(x, self.gate.weight, self.up.weight, self.down.weight, self.gate.bias, self.up.bias, self.down.bias,
-                                  activation=self.activation)
+        args = [x, self.gate.weight, self.up.weight, self.down.weight, self.gate.bias, self.up.bias, self.down.bias]
+        dtype = autocast_type()
+        if dtype is not None:
+            args = [None if t is None else t.to(dtype) for t in args]
+        return gated_feed_forward(*args, activation=self.activation)

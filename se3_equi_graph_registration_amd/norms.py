@@ -6,7 +6,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from .ops import context_ops, need_float
+from .ops import autocast_type, context_ops, need_float
 
 KINDS = ("layer", "rms")
 _MAX_WIDTH = 8192
@@ -66,7 +66,8 @@ def residual_norm(x, f, pre_weight=None, pre_bias=None, *, post_weight=None, pos
 class ResidualNorm(nn.Module):
     """``residual_norm`` with its parameters: ``forward(x, f=None, gate=None) -> (y, u)``.  ``post`` / ``pre``: the norm behind the block and
     the one before the next; ``residual_scale``: start value of a trainable scale per channel (None: no scale).  In the first step of a
-    stack (``f=None``) the norm behind a block, the gate and the scale play no part."""
+    stack (``f=None``) the norm behind a block, the gate and the scale play no part.  Under ``torch.autocast`` ``f`` and ``gate`` may be of
+    another type than ``x`` and are taken in that of ``x``."""
 
     def __init__(self, width, kind="layer", post=True, pre=True, residual_scale=None, eps=1e-5):
         super().__init__()
@@ -83,5 +84,7 @@ class ResidualNorm(nn.Module):
     def forward(self, x, f=None, gate=None):
         if f is None:
             return residual_norm(x, None, self.pre_weight, self.pre_bias, kind=self.kind, eps=self.eps)
+        if autocast_type() is not None:
+            f, gate = f.to(x.dtype), None if gate is None else gate.to(x.dtype)
         return residual_norm(x, f, self.pre_weight, self.pre_bias, post_weight=self.post_weight, post_bias=self.post_bias, gate=gate,
                              scale=self.scale, kind=self.kind, eps=self.eps)

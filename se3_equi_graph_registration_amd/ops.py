@@ -59,6 +59,11 @@ def need_float(t, name, like=None, ndim=None):
     return t
 
 
+def autocast_type():
+    """The type that ``torch.autocast`` gives products on the device, or None outside it."""
+    return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else None
+
+
 def context_ops():
     """``torch.ops.equigspr`` (csrc/torch_context_ops.cpp): the context operators with their autograd nodes."""
     global _CONTEXT_OPS

@@ -177,3 +177,42 @@ def test_feed_forward_fp16_gradients_of_any_size(rows):
         g16, beyond, inside = got[n].cpu().double(), val[n].abs() - bound > 65520, val[n].abs() + bound < 65504
         assert (g16[beyond] == val[n].sign()[beyond] * float("inf")).all() and inside.sum() > 0.9 * inside.numel(), n
         within({n: torch.where(inside, g16, 0.0)}, {n: torch.where(inside, val[n], 0.0)}, {n: bound}, "feed_forward fp16, large gradients")
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("how", ["autocast", "parameters"])
+def test_context_in_16_bits(dtype, how):
+    """CloudContext behind an fp32 network in 16 bits, by autocast and by the type of its parameters: fp32 features in and out, and the fp64
+    blocks' values and gradients up to the roundings (about 8 a block, three blocks, each passed on at most doubled: 48 half steps)."""
+    from tests.test_gpu_context_model import _plain_context
+    torch.manual_seed(48)
+    ctx = pkg().CloudContext(32, num_heads=4, residual_scale=0.7, device="cuda")
+    if how == "parameters":
+        ctx = ctx.to(dtype)
+    h, grad = torch.randn(2, 2, 90, 32), torch.randn(2, 2, 90, 32)
+    hd = h.cuda().requires_grad_(True)
+    with torch.autocast("cuda", dtype=dtype, enabled=how == "autocast"):
+        out = ctx(hd)
+    assert out.dtype == torch.float32
+    got = torch.autograd.grad(out, [hd] + list(ctx.parameters()), grad.cuda())
+    assert all(g.dtype == p.dtype for g, p in zip(got[1:], ctx.parameters()))
+    ref, leaf, p = _plain_context(ctx, h)
+    want = torch.autograd.grad(ref, [leaf] + list(p.values()), grad.double())
+    for name, a, b in zip(["out", "h"] + list(p), [out] + list(got), [ref] + list(want)):
+        off, size = float((a.detach().cpu().double() - b.detach()).abs().max()), float(b.detach().abs().max())
+        assert off <= 48 * orc.half_step(dtype) * size, (name, off, size)
+
+
+def test_modules_under_autocast_run_in_its_type():
+    """The layers behave like nn.Linear under autocast: products in its type; the residual step keeps the type of the stream it adds to."""
+    x = torch.randn(2, 30, 32, device="cuda")
+    att, ff, norm = pkg().CloudAttention(32).cuda(), pkg().GatedFeedForward(32, 64).cuda(), pkg().ResidualNorm(32).cuda()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        a, f = att(x), ff(x)
+        y, u = norm(x, a)
+    assert (a.dtype, f.dtype, y.dtype, u.dtype) == (torch.bfloat16, torch.bfloat16, torch.float32, torch.float32)
+    low = [None if p is None else p.bfloat16() for p in (ff.gate.weight, ff.up.weight, ff.down.weight, ff.gate.bias, ff.up.bias, ff.down.bias)]
+    assert torch.equal(f, pkg().gated_feed_forward(x.bfloat16(), *low))
+    with torch.autocast("cuda", dtype=torch.bfloat16):                     # the operators themselves take what they are given
+        with pytest.raises(RuntimeError):
+            pkg().residual_norm(x, a)
