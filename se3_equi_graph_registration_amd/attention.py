@@ -10,7 +10,7 @@ import math
 import torch
 from torch import nn
 
-from .ops import context_ops, need_float
+from .ops import autocast_type, context_ops, need_float
 
 
 def _rows(t):
@@ -87,8 +87,12 @@ class CloudAttention(nn.Module):
     def forward(self, h, other=None, *, q_lens=None, kv_lens=None, key_mask=None):
         other = h if other is None else other
         b, n, _ = h.shape
-        q = self.to_q(h).view(b, n, self.num_heads, self.head_dim)
-        k = self.to_k(other).view(b, other.shape[1], self.kv_heads, self.head_dim)
-        v = self.to_v(other).view(b, other.shape[1], self.kv_heads, self.head_dim)
+        dtype = autocast_type()
+        # under autocast the casts are made here: its own keep a weight's copy for as long as the context lasts, past the optimizer's update
+        # when the context is around a loop, and out of reach of a captured step
+        project = lambda layer, x: layer(x) if dtype is None else nn.functional.linear(x.to(dtype), layer.weight.to(dtype))  # noqa: E731
+        q = project(self.to_q, h).view(b, n, self.num_heads, self.head_dim)
+        k = project(self.to_k, other).view(b, other.shape[1], self.kv_heads, self.head_dim)
+        v = project(self.to_v, other).view(b, other.shape[1], self.kv_heads, self.head_dim)
         out = cloud_attention(q, k, v, q_lens=q_lens, kv_lens=kv_lens, key_mask=key_mask)
-        return self.to_out(out.view(b, n, self.width))
+        return project(self.to_out, out.view(b, n, self.width))

@@ -18,7 +18,8 @@ class CloudContext(nn.Module):
     """``forward(h [2, B, N, width], valid=None) -> [2, B, N, width]``: ``h[0]`` / ``h[1]`` the point features of the source / target clouds.
     ``valid`` (bool ``[2, B, N]``): points that exist; the others are not looked at.  ``residual_scale`` starts the blocks near the
     identity.  The blocks run in the type of their parameters (``CloudContext(...).bfloat16()`` behind an fp32 EGNN), or, their products, in
-    that of ``torch.autocast``; the result has the type of ``h``."""
+    that of ``torch.autocast``; the result has the type of ``h``.  (``train.make_optimizer`` keeps every parameter in fp32: train in 16 bits
+    under autocast.)"""
 
     def __init__(self, width, n_layers=1, num_heads=4, hidden=None, kind="layer", activation="silu", residual_scale=0.1, device="cuda:0"):
         super().__init__()

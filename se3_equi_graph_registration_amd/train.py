@@ -1063,10 +1063,11 @@ def run_training_batches(model, batches, optimizer, step_loss, device, epoch=0, 
 
 
 def graphed_step_for(model, optimizer, k=16, loss_mode="3dmatch", **kw) -> "GraphedStep":
-    """The ``GraphedStep`` of ``(model, optimizer, k, loss_mode)``, created on first use and kept on the optimizer (its captured
-    graphs hold pointers into the optimizer's buckets)."""
+    """The ``GraphedStep`` of ``(model, optimizer, k, loss_mode)`` and of the type that ``torch.autocast`` sets around this call (a captured
+    step keeps the types it was recorded with), created on first use and kept on the optimizer (its captured graphs hold pointers into
+    the optimizer's buckets)."""
     cache = optimizer.__dict__.setdefault("_graphed_steps", {})
-    key = (id(model), int(k), loss_mode)
+    key = (id(model), int(k), loss_mode, ops.autocast_type())
     if key not in cache:
         cache[key] = GraphedStep(model, optimizer, k=k, loss_mode=loss_mode, **kw)
     return cache[key]
@@ -1201,8 +1202,8 @@ def evaluate_model(checkpoint_path, save_dir, model, dataloader, device, use_poi
         graph = not use_pointnet and os.environ.get("EQUIGSPR_EAGER_TRAINING") != "1"
     if graph:
         if not isinstance(graph, GraphedEval):
-            cache = model.__dict__.setdefault("_graphed_eval", {})
-            graph = cache.get((int(k), float(tau))) or cache.setdefault((int(k), float(tau)), GraphedEval(model, k=k, tau=tau))
+            cache, key = model.__dict__.setdefault("_graphed_eval", {}), (int(k), float(tau), ops.autocast_type())
+            graph = cache.get(key) or cache.setdefault(key, GraphedEval(model, k=k, tau=tau))
         table = graph.run(dataloader.loader if isinstance(dataloader, DeviceBatches) else dataloader)
         vals = table[:, [0, 1, 2, 4]].numpy()
     else:

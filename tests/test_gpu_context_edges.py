@@ -216,3 +216,37 @@ def test_modules_under_autocast_run_in_its_type():
     with torch.autocast("cuda", dtype=torch.bfloat16):                     # the operators themselves take what they are given
         with pytest.raises(RuntimeError):
             pkg().residual_norm(x, a)
+
+
+def test_autocast_around_a_loop_takes_every_update():
+    """One autocast context around several steps (a training loop): every call uses the weights as they are then, none a copy in the lower
+    type from an earlier call."""
+    x = torch.randn(2, 30, 32, device="cuda")
+    for module in (pkg().CloudAttention(32).cuda(), pkg().GatedFeedForward(32, 64).cuda()):
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            module(x)
+            with torch.no_grad():
+                for p in module.parameters():
+                    p.mul_(1.5)
+            again = module(x)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            assert torch.equal(again, module(x))
+
+
+def test_training_under_autocast_graphed_equals_eager():
+    """The package's training loop under autocast: the captured step gives the eager loop's weights bit for bit, and every parameter of the
+    blocks moves."""
+    from se3_equi_graph_registration_amd import train
+    from tests.test_gpu_context_model import _assert_same, _batches, _model, _state
+    batches = _batches(pkg(), 6)
+    m_e, m_g = _model(pkg()), _model(pkg())
+    start = {k: v.detach().clone() for k, v in m_e.context.named_parameters()}
+    o_e, o_g = train.make_optimizer(m_e, lr=1e-3), train.make_optimizer(m_g, lr=1e-3)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        train.train_one_epoch(m_e, batches, o_e, "cuda", 0, log_interval=0, k=8, graph=False)
+        train.train_one_epoch(m_g, batches, o_g, "cuda", 0, log_interval=0, k=8)
+        assert train.graphed_step_for(m_g, o_g, k=8).steps_replayed == 5
+    assert train.graphed_step_for(m_g, o_g, k=8).steps_replayed == 0       # outside autocast another step, recorded in fp32
+    _assert_same(_state(m_e, o_e), _state(m_g, o_g))
+    for k, v in m_e.context.named_parameters():
+        assert not torch.equal(v.detach(), start[k]), k
