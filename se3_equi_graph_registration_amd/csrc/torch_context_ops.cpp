@@ -10,6 +10,9 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
+#include <unordered_set>
+#include <vector>
+
 #include "../../include/equigspr.h"
 
 namespace {
@@ -42,21 +45,34 @@ void need(const at::Tensor& t, const at::Tensor& like, const char* name, bool de
     TORCH_CHECK(!dense || t.is_contiguous(), "equigspr: ", name, " must be contiguous");
 }
 
-// Whether a backward that is recorded into a hipGraph from here on would reach into work of another stream: `t` belongs to an autograd graph
-// -- or, a leaf, hangs on the gradient accumulator of one -- that was built on a stream that is not being captured.  The autograd engine
-// would synchronise with that stream during the capture, which ends the process; the ops raise instead.
-bool grad_lives_on_other_stream(const at::Tensor& t) {
-    if (!t.defined() || !t.is_cuda() || !t.requires_grad()) return false;
-    const std::shared_ptr<torch::autograd::Node> node = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
-    if (!node) return false;
-    const auto stream = node->stream();
+// Whether a backward that is recorded into a hipGraph from here on would reach into work of another stream: `t` -- or anything before it in
+// its autograd graph, down to the leaves' gradient accumulators, which an eager graph of the same leaves keeps alive -- was built on a stream
+// that is not being captured.  The autograd engine would synchronise with that stream during the capture, which ends the process; the ops
+// raise instead.  Walked only while a call is being recorded.
+bool node_on_other_stream(torch::autograd::Node& node, hipStream_t now) {
+    const auto stream = node.stream();
     if (!stream.has_value()) return false;
     const c10::hip::HIPStreamMasqueradingAsCUDA other(*stream);      // autograd's streams carry the masqueraded device type
-    if (other.stream() == stream_of(t)) return false;
+    if (other.stream() == now) return false;
     if (other.stream() == nullptr) return true;                     // the default stream is never part of a capture
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(other.stream(), &status) != hipSuccess) { (void)hipGetLastError(); return true; }
     return status != hipStreamCaptureStatusActive;
+}
+bool grad_lives_on_other_stream(const at::Tensor& t) {
+    if (!t.defined() || !t.is_cuda() || !t.requires_grad()) return false;
+    const hipStream_t now = stream_of(t);
+    const std::shared_ptr<torch::autograd::Node> first = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
+    std::vector<torch::autograd::Node*> open = {first.get()};        // first keeps everything behind it alive
+    std::unordered_set<torch::autograd::Node*> seen;
+    while (!open.empty()) {
+        torch::autograd::Node* const node = open.back();
+        open.pop_back();
+        if (!node || !seen.insert(node).second) continue;
+        if (node_on_other_stream(*node, now)) return true;
+        for (const auto& edge : node->next_edges()) open.push_back(edge.function.get());
+    }
+    return false;
 }
 // true if one of the inputs wants a gradient; refuses a capture that would end the process, and tangents, which the output would lose
 bool training(std::initializer_list<at::Tensor> inputs) {

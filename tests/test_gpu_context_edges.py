@@ -250,3 +250,43 @@ def test_training_under_autocast_graphed_equals_eager():
     _assert_same(_state(m_e, o_e), _state(m_g, o_g))
     for k, v in m_e.context.named_parameters():
         assert not torch.equal(v.detach(), start[k]), k
+
+
+@pytest.mark.parametrize("layer", ["attention", "feed forward behind a product"])
+def test_capture_beside_a_living_eager_graph_is_refused_through_a_module(layer):
+    """An eager graph that is still alive and shares only parameters that lie behind other operations: recording the call is refused there,
+    too.  Without that graph, it records forward and backward."""
+    x = torch.randn(2, 40, 32, device="cuda")
+    if layer == "attention":
+        module = pkg().CloudAttention(32).cuda()
+    else:
+        lin, w = torch.nn.Linear(32, 32).cuda(), [torch.randn(64, 32, device="cuda"), torch.randn(64, 32, device="cuda"), torch.randn(32, 64, device="cuda")]
+        module = lambda t: pkg().gated_feed_forward(lin(t), *w)  # noqa: E731
+    weight = module.to_q.weight if layer == "attention" else lin.weight
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):                                          # libraries set themselves up outside the recording
+        torch.autograd.grad(module(x).sum(), weight)
+    torch.cuda.current_stream().wait_stream(side)
+    alive = module(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x * 2
+        with pytest.raises(RuntimeError, match="still alive"):
+            module(x)
+        with torch.no_grad():
+            out = module(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    torch.testing.assert_close(out, alive.detach(), rtol=1e-6, atol=1e-6)  # the products before may come from another library kernel
+    del alive
+    graph2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph2):
+        grad, = torch.autograd.grad(module(x), weight, torch.ones_like(out))
+    for _ in range(3):
+        grad.zero_()
+        graph2.replay()
+        torch.cuda.synchronize()
+        want, = torch.autograd.grad(module(x), weight, torch.ones_like(out))
+        torch.testing.assert_close(grad, want, rtol=1e-5, atol=1e-5 * float(want.abs().max()))
