@@ -161,7 +161,9 @@ static inline AttnTensor<T> attn_tensor(const equigspr_attention_tensor& t, int 
 
 // rows of a tile lie within 2^31 bytes of each other (the kernels' 32-bit offsets inside a tile)
 static inline bool attn_near(const equigspr_attention_tensor& t, int esize) {
-    return (t.stride_point * 128 + t.stride_head * 128) * esize < (1ll << 31) && t.stride_batch >= 0 && t.stride_point >= 0 && t.stride_head >= 0;
+    const int64_t most = 1ll << 31;           // of each first: the sum must not wrap around
+    if (t.stride_batch < 0 || t.stride_point < 0 || t.stride_head < 0 || t.stride_point >= most || t.stride_head >= most) return false;
+    return (t.stride_point + t.stride_head) * 128 * esize < most;
 }
 
 // checks the description and derives what the kernels use; 0 or an error code
