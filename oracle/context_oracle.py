@@ -4,7 +4,8 @@ type.  Checker only.  The operators have no counterpart in the reference ("parit
 import torch
 
 F32 = 2.0 ** -24
-# fp32 inputs: products of three bf16 planes each, three of nine products dropped, below 2^-22 |a b| together with the rest
+# fp32 inputs: products of three bf16 planes each; the three of nine products that are dropped are below 2^-22 |a b|, and as much again is
+# allowed for the rest (the partial sums' rounding inside the matrix pipe)
 PLANES = {torch.float32: 2.0 ** -21, torch.bfloat16: 0.0, torch.float16: 0.0}
 
 

@@ -4,8 +4,9 @@
 // l & 31 and rows 8 (r >> 2) + 4 (l >> 5) + (r & 3), r = 0..15; an A or B operand is eight consecutive k at 8 (l >> 5) of row l & 31).
 //   bf16, fp16   one plane: the value itself.
 //   fp32         three bf16 planes, x = hi + mid + lo (8 significant bits each, exact to 24), and the six products hi.hi, hi.mid,
-//                mid.hi, mid.mid, hi.lo, lo.hi: the three dropped ones are below 2^-22 |a b| and average 2^-24, what an fp32 product
-//                rounds.  Six passes of the 16-bit pipe cost 6/16 of the fp32 matrix instruction's time (2.5 against 0.157 PFLOP/s).
+//                mid.hi, mid.mid, hi.lo, lo.hi.  hi is cut off (to nearest, the largest values would become infinite), mid rounded to
+//                nearest: lo has either sign and is below 2^-16 |x|, so the three dropped products are below 2^-22 |a b| and average
+//                to zero (with mid cut off, too: 2^-21, always towards zero, 0.7 x 2^-24 on average).  Six passes of the 16-bit pipe cost 6/16 of the fp32 matrix instruction's time (2.5 against 0.157 PFLOP/s).
 //                A non-finite fp32 value gives non-finite results (its residual planes are NaN).
 // Values are kept as raw 16-bit lanes (short vectors) and cast at the instruction.
 #pragma once
@@ -61,16 +62,15 @@ __device__ __forceinline__ void mma(pf32x16& acc, const Op8<T>& a, const Op8<T>&
     acc = mfma32<T>(a.p[0], b.p[0], acc);
 }
 
-// two fp32 -> the planes' packed 16-bit pairs.  fp32: truncation, so that hi + mid + lo is the value exactly.
+// two fp32 -> the planes' packed 16-bit pairs.  fp32: hi + mid + lo is the value exactly.
 template <int T>
 __device__ __forceinline__ void split2(float x, float y, unsigned (&out)[Num<T>::planes]) {
     if constexpr (T == kF32) {
         const unsigned ux = __float_as_uint(x), uy = __float_as_uint(y);
         out[0] = __builtin_amdgcn_perm(uy, ux, 0x07060302u);
         const float rx = x - __uint_as_float(ux & 0xffff0000u), ry = y - __uint_as_float(uy & 0xffff0000u);
-        const unsigned vx = __float_as_uint(rx), vy = __float_as_uint(ry);
-        out[1] = __builtin_amdgcn_perm(vy, vx, 0x07060302u);
-        const float sx = rx - __uint_as_float(vx & 0xffff0000u), sy = ry - __uint_as_float(vy & 0xffff0000u);
+        out[1] = __builtin_bit_cast(unsigned, __builtin_convertvector((pf32x2){rx, ry}, pbf16x2));
+        const float sx = rx - __uint_as_float(out[1] << 16), sy = ry - __uint_as_float(out[1] & 0xffff0000u);
         out[2] = __builtin_amdgcn_perm(__float_as_uint(sy), __float_as_uint(sx), 0x07060302u);
     } else if constexpr (T == kBF16) {
         out[0] = __builtin_bit_cast(unsigned, __builtin_convertvector((pf32x2){x, y}, pbf16x2));

@@ -290,3 +290,15 @@ def test_capture_beside_a_living_eager_graph_is_refused_through_a_module(layer):
         torch.cuda.synchronize()
         want, = torch.autograd.grad(module(x), weight, torch.ones_like(out))
         torch.testing.assert_close(grad, want, rtol=1e-5, atol=1e-5 * float(want.abs().max()))
+
+
+@pytest.mark.parametrize("rows", [4, 200])
+def test_feed_forward_fp32_products_keep_their_last_bits(rows):
+    """y = relu(x w) with x = w = 1 + 2^-7 - 2^-23, whose parts below 8 and 16 bits are as large as they can be.  Split to nearest they are
+    1, 2^-7 and -2^-23, and what a product leaves out is below 2^-28; two products follow each other (the second with 1), each rounds its
+    sum once by up to 2^-23, the small parts' sums below 2^-28: 5 x 2^-24 in all."""
+    a = 1 + 2.0 ** -7 - 2.0 ** -23
+    c = lambda *s, v=a: torch.full(s, v, device="cuda")  # noqa: E731
+    y = pkg().gated_feed_forward(c(rows, 1), c(1, 1), c(1, 1, v=0.0), c(1, 1, v=1.0), b_up=c(1, v=1.0), activation="relu")
+    off = float((y.double() / a ** 2 - 1).abs().max())
+    assert off <= 5 * 2.0 ** -24, off * 2 ** 24
