@@ -408,7 +408,9 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(const float* part0, const
 }
 
 // Parts: the owned axis alone gives too few workgroups when it is short, and a causal mask leaves the first keys with all the work, so the
-// other axis is cut until there are two workgroups per compute unit (causal: four), into parts of at least 256.
+// other axis is cut until there are two workgroups per compute unit (causal: four), one part for every 256 of
+// its length at most (257 are cut into 192 and 65; with whole parts of 256 alone, fp32 heads of 8 at 2 x 300^2 took 51 us instead of 44, heads of
+// 32 at 2 x 700^2 73 instead of 64).
 static int attn_bwd_splits(int64_t tiles, int64_t length, int64_t want) {
     if (tiles == 0 || tiles >= want) return 1;
     const int64_t most = (length + 255) / 256, s = want / tiles;

@@ -143,6 +143,8 @@ constexpr int kAttnMaxDim = 128;
 
 // rows of a staged tile: 64, except where three planes of a wide head would take too much LDS
 template <int T, int W> constexpr int attn_tile() { return T == kF32 && W > 32 ? 32 : 64; }
+// the same for a head dim, on the host (W is 32 up to 32 dims)
+static inline int attn_tile_of(int dtype, int dim) { return dtype == kF32 && dim > 32 ? 32 : 64; }
 
 // ---- host side
 // f<T, W, KS>: the head dim in steps of 16, in tiles of 32, 64 or 128 columns (dims up to 16 and up to 96 skip the empty steps)
