@@ -67,19 +67,22 @@ __device__ __forceinline__ float ff_held(const float* range) {
     return ldexpf(1.f, e < -4 ? -4 - e : e >= 4 ? 3 - e : 0);
 }
 template <int T>
-__global__ __launch_bounds__(256) void ff_range_kernel(const typename Num<T>::type* x, int64_t n, float* range) {
+__global__ __launch_bounds__(1024) void ff_range_kernel(const typename Num<T>::type* x, int64_t n, float* range) {
     float m = 0.f;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)kFfRange * 256 * 8) {
+    for (int64_t i = ((int64_t)blockIdx.x * 1024 + threadIdx.x) * 8; i < n; i += (int64_t)kFfRange * 1024 * 8) {
         float v[8];
         load8f<T>(x + i, n - i < 8 ? (int)(n - i) : 8, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]));
     }
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    __shared__ float part[4];
+    __shared__ float part[16];
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
     __syncthreads();
-    if (threadIdx.x == 0) range[blockIdx.x] = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    if (threadIdx.x) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) m = fmaxf(m, part[i]);
+    range[blockIdx.x] = m;
 }
 
 // act(z) and its derivative
@@ -662,7 +665,7 @@ static int ff_backward(const equigspr_gated_feed_forward* d, const void* gy, con
     g.act = d->activation;
     const float* range = nullptr;
     if constexpr (T == kF16) {                // the first floats of the workspace
-        ff_range_kernel<T><<<kFfRange, 256, 0, st>>>((const E*)gy, (int64_t)r * out, work);
+        ff_range_kernel<T><<<kFfRange, 1024, 0, st>>>((const E*)gy, (int64_t)r * out, work);
         EQ_CHECK_LAUNCH("gated_feed_forward_backward (range)");
         range = work;
         work += kFfRange;
