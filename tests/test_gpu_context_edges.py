@@ -302,3 +302,24 @@ def test_feed_forward_fp32_products_keep_their_last_bits(rows):
     y = pkg().gated_feed_forward(c(rows, 1), c(1, 1), c(1, 1, v=0.0), c(1, 1, v=1.0), b_up=c(1, v=1.0), activation="relu")
     off = float((y.double() / a ** 2 - 1).abs().max())
     assert off <= 5 * 2.0 ** -24, off * 2 ** 24
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("b,n,c,gate", [
+    (1, 4200, 520, None), (1, 4200, 521, None), (1, 70000, 24, None), (1, 2100, 4100, None),      # several rows per workgroup, forward and backward
+    (2, 500, 40, "all"), (2, 450, 700, "all"), (800, 3, 16, "sample"),                            # several units per workgroup
+    (3, 777, 100, "sample"), (3, 1001, 600, "sample"), (2, 1001, 4100, "sample"), (1, 3001, 600, "one")])      # a unit cut at the end of its gate row
+def test_residual_norm_more_than_one_trip(dtype, kind, b, n, c, gate):
+    """The loops over a workgroup's rows and units: the next row's loads, sums carried over rows, two buffers for the row sums in turn."""
+    residual_norm_case(51, dtype, kind, b, n, c, gate=gate)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("b,h,hk", [(11, 6, 3), (7, 10, 10), (33, 2, 1)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_more_than_32_heads_in_a_batch(dtype, b, h, hk, causal):
+    """More (sample, key head) pairs than one group of workgroups takes, ragged."""
+    g = torch.Generator().manual_seed(52)
+    lens = lambda n: torch.randint(0, n + 1, (b,), generator=g).tolist()  # noqa: E731
+    attention_case(53, dtype, b, 140, 200, h, hk, 16, causal, lens(140), lens(200))
