@@ -82,13 +82,6 @@ struct Stager {
             raw[u] = row ? load8<T>(row, (id % kChunks) * 8, width) : raw_zero<T>();
         }
     }
-    // rows r with gone(r) become zeros, whatever was loaded
-    template <class F>
-    __device__ __forceinline__ void drop(F gone) {
-#pragma unroll
-        for (int u = 0; u < kPer; ++u)
-            if (gone((int)(threadIdx.x + u * NT) / kChunks)) raw[u] = raw_zero<T>();
-    }
     __device__ __forceinline__ void store(short* tile) const {
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
