@@ -40,8 +40,9 @@ def cloud_attention(q, k, v, *, q_lens=None, kv_lens=None, key_mask=None, causal
 
     A point without a visible key, and a point behind ``q_lens``, gives zeros and takes no gradient.  Keys hidden by ``kv_lens`` or
     ``key_mask`` are never used, whatever they hold, and their gradients are zero; a key that ``causal`` hides from some points only has
-    weight zero there, so its values must be finite.  Differentiable once in q, k and v (reverse mode; tangents are refused); bitwise reproducible (no atomics).
-    Scores, probabilities' sums and gradients' sums are fp32."""
+    weight zero there, so its values must be finite.  A NaN that a point sees reaches its output and every gradient of its keys; in float32
+    an infinity in k or v does so as NaN.  Differentiable once in q, k and v (reverse mode; tangents are refused); bitwise reproducible (no
+    atomics).  Scores, probabilities' sums and gradients' sums are fp32."""
     need_float(q, "q", ndim=4)
     need_float(k, "k", like=q, ndim=4)
     need_float(v, "v", like=q, ndim=4)
@@ -90,7 +91,9 @@ class CloudAttention(nn.Module):
         dtype = autocast_type()
         # under autocast the casts are made here: its own keep a weight's copy for as long as the context lasts, past the optimizer's update
         # when the context is around a loop, and out of reach of a captured step
-        project = lambda layer, x: layer(x) if dtype is None else nn.functional.linear(x.to(dtype), layer.weight.to(dtype))  # noqa: E731
+        project = lambda layer, x: layer(x) if dtype is None else nn.functional.linear(x, layer.weight.to(dtype))  # noqa: E731
+        if dtype is not None:
+            h, other = h.to(dtype), other.to(dtype)
         q = project(self.to_q, h).view(b, n, self.num_heads, self.head_dim)
         k = project(self.to_k, other).view(b, other.shape[1], self.kv_heads, self.head_dim)
         v = project(self.to_v, other).view(b, other.shape[1], self.kv_heads, self.head_dim)

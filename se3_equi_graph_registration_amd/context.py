@@ -12,14 +12,17 @@ from torch import nn
 from .attention import CloudAttention
 from .feedforward import GatedFeedForward
 from .norms import ResidualNorm
+from .ops import need_float
 
 
 class CloudContext(nn.Module):
     """``forward(h [2, B, N, width], valid=None) -> [2, B, N, width]``: ``h[0]`` / ``h[1]`` the point features of the source / target clouds.
-    ``valid`` (bool ``[2, B, N]``): points that exist; the others are not looked at.  ``residual_scale`` starts the blocks near the
-    identity.  The blocks run in the type of their parameters (``CloudContext(...).bfloat16()`` behind an fp32 EGNN), or, their products, in
-    that of ``torch.autocast``; the result has the type of ``h``.  (``train.make_optimizer`` keeps every parameter in fp32: train in 16 bits
-    under autocast.)"""
+    ``valid`` (bool ``[2, B, N]``): points that exist; the others are not attended to (their own rows are computed all the same, so they
+    must be finite: zeros, not NaN).  ``residual_scale`` starts the blocks near the identity.
+
+    The blocks run in the type of their parameters (``CloudContext(...).bfloat16()`` behind an fp32 EGNN), or, their products, in that of
+    ``torch.autocast``; the result has the type of ``h``.  (``train.make_optimizer`` keeps every parameter in fp32: train in 16 bits under
+    autocast.)"""
 
     def __init__(self, width, n_layers=1, num_heads=4, hidden=None, kind="layer", activation="silu", residual_scale=0.1, device="cuda:0"):
         super().__init__()
@@ -38,6 +41,7 @@ class CloudContext(nn.Module):
     def forward(self, h, valid=None):
         if h.dim() != 4 or h.shape[0] != 2 or h.shape[3] != self.width:
             raise RuntimeError(f"CloudContext: expected h [2, B, N, {self.width}], got {tuple(h.shape)}")
+        need_float(h, "h")
         _, b, n, c = h.shape
         if valid is not None and (valid.dtype != torch.bool or valid.shape != (2, b, n)):
             raise RuntimeError(f"valid: expected bool [2, {b}, {n}], got {valid.dtype} {tuple(valid.shape)}")

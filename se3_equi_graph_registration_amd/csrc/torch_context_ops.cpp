@@ -120,7 +120,7 @@ equigspr_attention describe(const at::Tensor& q, const at::Tensor& k, const at::
                             bool causal, double scale) {
     equigspr_attention d = {};
     d.dtype = dtype_code(q);
-    for (int i = 0; i < 3; ++i) TORCH_CHECK(counted(q.size(i)) && counted(k.size(i)), "equigspr::cloud_attention: sizes out of range");
+    for (int i = 0; i < 4; ++i) TORCH_CHECK(counted(q.size(i)) && counted(k.size(i)), "equigspr::cloud_attention: sizes out of range");
     d.batch = (int32_t)q.size(0); d.nq = (int32_t)q.size(1); d.nk = (int32_t)k.size(1);
     d.heads = (int32_t)q.size(2); d.kv_heads = (int32_t)k.size(2); d.dim = (int32_t)q.size(3);
     d.causal = causal;

@@ -18,8 +18,8 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
     (exact) or "relu".  Products accumulate in fp32; the hidden layer is held in the inputs' dtype between the two products, as are the
     projections' gradients in the backward.  In float16 the hidden layer must stay within that type's range; the projections' gradients are
     held relative to the largest output gradient, must stay within 2^12 times it and lose bits below 2^-10 of it.  The backward keeps both
-    projections in float32.  Up to 8 388 480 rows a call.  Differentiable once in every
-    tensor (reverse mode; tangents are refused); bitwise reproducible (no atomics)."""
+    projections in float32.  In float32 an infinity in a product's operand gives NaN.  Up to 8 388 480 rows a call.  Differentiable once in
+    every tensor (reverse mode; tangents are refused); bitwise reproducible (no atomics)."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"gated_feed_forward: activation {activation!r}, expected one of {sorted(ACTIVATIONS)}")
     need_float(x, "x")

@@ -323,3 +323,14 @@ def test_attention_more_than_32_heads_in_a_batch(dtype, b, h, hk, causal):
     g = torch.Generator().manual_seed(52)
     lens = lambda n: torch.randint(0, n + 1, (b,), generator=g).tolist()  # noqa: E731
     attention_case(53, dtype, b, 140, 200, h, hk, 16, causal, lens(140), lens(200))
+
+
+def test_other_types_and_widths_are_refused():
+    """What the operators' checks refuse, the modules and the dispatcher ops refuse, too: a module does not cast a type that they do not take."""
+    ctx = pkg().CloudContext(32, device="cuda")
+    for h in (torch.zeros(2, 1, 8, 32, dtype=torch.float64, device="cuda"), torch.zeros(2, 1, 8, 32, dtype=torch.int64, device="cuda")):
+        with pytest.raises(RuntimeError, match="expected float32"):
+            ctx(h)
+    wide = torch.empty(1, 1, 1, 2 ** 32 + 8, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="range"):
+        torch.ops.equigspr.cloud_attention(wide, wide, wide, None, None, None, False, 1.0)
