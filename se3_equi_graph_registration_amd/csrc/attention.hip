@@ -8,9 +8,11 @@
 // drops, fp32 keeps all three).
 // Few rows against many keys: the key axis is split over workgroups, each writes its normalised part and its log-sum, and
 // attn_join_kernel joins them in split order (no atomics: results do not depend on timing).
-// Bound: the vector ALU up to heads of 64 (160 instructions of softmax per 16 products of a 64-key tile), the matrix pipe at 128.  Measured,
-// bf16: 8 x 2048^2 x 8 heads of 64 104 us (660 TFLOP/s), 8192^2 x 16 heads of 128 590 us (930), one token against 16 x 16384 keys of 8 heads
-// of 128 156 us (5.3 TB/s); fp32: 2 x 4096^2 x 4 heads of 32 113 us (150 TFLOP/s).
+// Bound: how little softmax and products overlap.  By counters, heads of 64: the vector ALU is busy 0.56 of the time, the matrix pipe 0.31 (a
+// 64-key tile costs a wave 160 instructions of softmax, 32 of them exponentials, beside 16 products), heads of 128: 0.44 and 0.44; a wave does
+// one after the other, and what the other waves of its SIMD fill in leaves the rest idle.  Few rows: HBM.  Measured, bf16: 8 x 2048^2 x 8 heads
+// of 64 104..110 us (625..660 TFLOP/s), 8192^2 x 16 heads of 128 575 us (955), one token against 16 x 16384 keys of 8 heads of 128 199 us with the
+// join (5.4 TB/s); fp32: 2 x 4096^2 x 4 heads of 32 110 us (156 TFLOP/s), the token's three planes per key 2.6 TB/s.
 #include "attention_device.h"
 
 namespace eq {

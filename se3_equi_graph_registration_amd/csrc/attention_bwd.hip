@@ -7,8 +7,10 @@
 // P and dS are rounded to the inputs' 16-bit type for those products (heads of up to 16 dims take a second plane with what that
 // drops), everything else is fp32; the forward leaves what the output's rounding dropped in a second plane for delta, whose error every
 // dS of the row would share.
-// Bound: as the forward, and the registers -- the accumulators of wide heads leave two waves per SIMD.  Measured, bf16: 8 x 2048^2 x 8 heads
-// of 64 340 us (505 TFLOP/s of the five products that the mathematics needs), 8192^2 x 16 / 4 heads of 128 2.0 ms (680), causal 1.14 ms.
+// Bound: as the forward (matrix pipe busy 0.31 / 0.36 at heads of 64 in the two kernels, 0.47 / 0.37 at 128), and the registers -- the
+// accumulators of wide heads leave two waves per SIMD, and the keys' kernel at 97..128 dims spills (bf16 43, fp16 28 registers, 80 bytes).
+// Measured, bf16: 8 x 2048^2 x 8 heads of 64 285 us (600 TFLOP/s of the five products that the mathematics needs), 8192^2 x 16 / 4 heads of 128
+// 2.0 ms (690), causal 1.15 ms.
 // fp16: dS is about 1/keys of the output gradient and would sink below fp16's range, so it is held as 2^E dS, with E from the largest
 // |dO| and |V| of the sample and key head such that the bound |dS| <= 2 dim max|dO| max|V| stays in range; undone in fp32 at the end.
 // (One E for a whole batch would let one sample's or head's large gradients push the others' into fp16's smallest steps.)

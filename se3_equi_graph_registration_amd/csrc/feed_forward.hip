@@ -10,7 +10,9 @@
 // inputs' type (one rounding each); z | u, which only the epilogue of the backward reads, stays fp32 -- in 16 bits its rounding would come
 // on top of dz's and du's in every gradient (bf16: 1.8 instead of 1.4 times the outputs' own rounding).
 // fp16: dz and du are held as 2^E dz and 2^E du, with E from the largest |dy| (ff_held), undone in fp32 where their products leave.
-// Bound: the matrix pipe for many rows, the weights' bytes for few.  Measured, bf16, 16384 x 1024 x 4096: projections 402 us (685 TFLOP/s,
+// Bound: for many rows the matrix pipe together with what does not run beside it -- it is busy 0.43..0.51 of the time in the plain products, 0.33
+// in the projections and 0.19 in the hidden gradients, whose epilogues (0.7 and 0.8 GB) run alone, one workgroup per compute unit; for few
+// rows the weights' bytes.  Measured, bf16, 16384 x 1024 x 4096: projections 402 us (685 TFLOP/s,
 // with 0.7 GB of results), output 147 (935), hidden gradients 330 (415, with 0.8 GB through its epilogue), input 276 (995), weights 300 + 161 (915, 855).
 #include "planes.h"
 

@@ -3,10 +3,12 @@
 //   norm = (v - mean) rsqrt(var + eps) w + b  (layer)  or  v rsqrt(mean(v^2) + eps) w  + b (rms).
 // One pass over memory: a row stays in the registers of L threads (8, 64, 256, 512 or 1024) from its loads to its stores, so the forward
 // moves x, f, y, u once and the backward x, f, grad_y, grad_u, grad_x, grad_f once -- the backward recomputes both norms from x and f
-// instead of reading anything the forward kept.  Bound: HBM forward
+// instead of reading anything the forward kept.  (The backward of widths above 4096 has 128 registers a thread and spills 77..147 of them:
+// 224..288 bytes of scratch; a few are spilled where odd widths cut the columns.)  Bound: HBM forward
 // (32768 x 2048 bf16: 111 us, 4.8 TB/s); backward the registers of its column sums, which leave two workgroups per compute unit (250 us,
-// 3.2 TB/s).  All sums are fp32, the spread is taken about the mean (two sums), y
-// enters the second norm before its rounding to the output type.
+// 3.2 TB/s), and above 4096 the spills (8192 x 8192 bf16: training 744 us, 156 of them forward).  A gate of x's shape makes every row
+// a unit with sums of its own: 131072 x 64 bf16, training, 650 us against 95 with a gate per sample, 32768 x 2048 448 against 293.
+// All sums are fp32, the spread is taken about the mean (two sums), y enters the second norm before its rounding to the output type.
 // Parameter gradients are column sums: every workgroup sums its rows in registers, norm_columns_kernel adds the workgroups' partial
 // rows in order.  The gate's gradient is a sum over the rows that share a gate row: a workgroup takes whole runs of them.
 #include "planes.h"
