@@ -334,3 +334,50 @@ def test_other_types_and_widths_are_refused():
     wide = torch.empty(1, 1, 1, 2 ** 32 + 8, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(RuntimeError, match="range"):
         torch.ops.equigspr.cloud_attention(wide, wide, wide, None, None, None, False, 1.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("c", [24, 33, 700, 5000])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_residual_norm_non_finite_row_stays_in_its_row(dtype, kind, c, value):
+    """A NaN or an infinity in one value of a row: that row's second norm and gradients are NaN (some of them, for the infinity), the other rows
+    are untouched, and the parameters' gradients show it."""
+    g = torch.Generator().manual_seed(54)
+    x, f, gy, gu = (normal(g, 2, 70, c, dtype=dtype).cuda() for _ in range(4))
+    w = [normal(g, c, dtype=torch.float32).cuda().requires_grad_(True) for _ in range(2)]
+
+    def run(bad):
+        a = [x.clone(), f.clone()]
+        if bad:
+            a[0][1, 33, c // 2] = value
+        a = [t.requires_grad_(True) for t in a]
+        y, u = pkg().residual_norm(a[0], a[1], w[0], post_weight=w[1], kind=kind)
+        return [y.detach(), u.detach()] + list(torch.autograd.grad((y, u), a + w, (gy, gu)))
+    clean, dirty = run(False), run(True)
+    rest = torch.ones(2, 70, dtype=torch.bool, device="cuda")
+    rest[1, 33] = False
+    for i, (p, q) in enumerate(zip(clean[:4], dirty[:4])):
+        assert torch.equal(p[rest], q[rest]), i
+        assert not q[1, 33].isfinite().all(), i
+    assert dirty[1][1, 33].isnan().any() and dirty[4].isnan().any() and dirty[5].isnan().any()
+    assert torch.equal(clean[0][1, 33, : c // 2], dirty[0][1, 33, : c // 2])      # the sum itself: this value only
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("rows", [5, 200])
+def test_feed_forward_infinity_in_a_row_stays_in_its_row(dtype, rows):
+    """An infinity in one row of x (16-bit types): the row's outputs are those of the formula, infinite or NaN, the other rows are untouched."""
+    g = torch.Generator().manual_seed(55)
+    x = normal(g, rows, 24, dtype=dtype)
+    w = [normal(g, 40, 24, dtype=dtype, scale=0.2), normal(g, 40, 24, dtype=dtype, scale=0.2), normal(g, 20, 40, dtype=dtype, scale=0.2)]
+    bad = x.clone()
+    bad[3, 5] = float("inf")
+    call = lambda t: pkg().gated_feed_forward(t.cuda(), *(v.cuda() for v in w), activation="relu").cpu()  # noqa: E731
+    clean, dirty = call(x), call(bad)
+    rest = torch.arange(rows) != 3
+    assert torch.equal(clean[rest], dirty[rest])
+    wg, wu, wd = (v.double() for v in w)
+    z, u = bad[3].double() @ wg.mT, bad[3].double() @ wu.mT
+    want = (z.clamp(min=0) * u) @ wd.mT                                    # 0 * inf in units that are off, inf - inf in the sum
+    assert torch.equal(dirty[3].isnan(), want.isnan()) and torch.equal(dirty[3].isinf(), want.isinf())
